@@ -448,6 +448,71 @@ int v7g_quantize_q8(int8_t *out_q, float *out_s, const float *x, int rows, int r
 int v7g_embedding_gather_q8(float *out, const int32_t *ids, int n_tokens, const int8_t *table_q,
                             const float *table_s, int dim, int vocab);
 
+/* ---------------------------------------------------------------------------
+ * 4. Around the K/V cache: attention, pages, token scores
+ *
+ * No counterpart in the reference's exports as these forms: its attention
+ * (v7d_attention, src/asm/forward_q8.inc:370, prefill_q8.inc:947) reads one
+ * sequence's contiguous cache, token by token.  Lengths, offsets, block tables
+ * and masks are read from device memory by the kernels, so a call never waits
+ * for the host and can be captured; what they hold is brought into the range
+ * of its buffer there (a wrong one gives wrong rows, never an access outside).
+ * ------------------------------------------------------------------------- */
+
+/* The binary16 K and V pages of a cache.  Token i of page p of layer l has its
+ * n_kv_heads heads of head_dim elements, contiguous, at
+ * k + l*layer_stride + p*page_stride + i*token_stride (v the same).  page_size
+ * is a power of two, 16..65536; strides in elements, multiples of 4; k and v
+ * 8-byte aligned.  A block table row [table_width] names the pages of a
+ * sequence's tokens in order, page_size tokens each; an entry outside
+ * [0, n_pages) is no page. */
+typedef struct v7g_kv_pages {
+    uint16_t *k, *v;
+    int n_layers, n_pages, page_size, n_kv_heads, head_dim;
+    long long layer_stride, page_stride, token_stride;
+} v7g_kv_pages;
+
+/* Causal attention over packed sequences with grouped heads: sequence b has
+ * the tokens cu_seqlens[b] .. cu_seqlens[b+1]-1 of q and out, and the K/V rows
+ * cu_seqlens_k[b] .. cu_seqlens_k[b+1]-1 (NULL: the same numbers); its token i
+ * of n attends to its rows j <= i + m - n of m, so with m > n the first m - n
+ * rows are what the cache already held.  head h of out and q (f32) reads KV
+ * head h / (n_q_heads / n_kv_heads) of k and v (binary16).  out = softmax(q . k
+ * * scale) v, accurate as f32 arithmetic is; a token that sees nothing gives
+ * zeros.  Tokens outside every sequence are left as they were; K/V rows no
+ * token sees may hold anything.  An infinite element of V that a token sees
+ * gives it NaN or infinity.
+ * q, out: head_dim contiguous heads per token, token strides in floats, % 4;
+ * k, v the same in binary16 elements, 8-byte aligned.  head_dim % 32 == 0 in
+ * [64, 512]; n_q_heads a multiple of n_kv_heads.  out overlaps nothing.
+ * workspace: v7g_attention_prefill_workspace(...) bytes (may be 0), 16-byte
+ * aligned; its contents are not kept from call to call, and calls that may run
+ * at the same time need their own. */
+int v7g_attention_prefill(float *out, long long out_stride, const float *q, long long q_stride, const uint16_t *k,
+                          long long k_stride, const uint16_t *v, long long v_stride, const int32_t *cu_seqlens,
+                          const int32_t *cu_seqlens_k, int n_seqs, int n_tokens, int n_kv_tokens, int n_q_heads,
+                          int n_kv_heads, int head_dim, float scale, void *workspace, int64_t workspace_bytes);
+int64_t v7g_attention_prefill_workspace(int n_seqs, int n_tokens, int n_kv_tokens, int n_q_heads, int n_kv_heads,
+                                        int head_dim);
+
+/* Attention of new tokens over a paged cache (layer 0 of pages): sequence b
+ * has context_lens[b] tokens in its pages, followed by the K/V rows of its new
+ * tokens, which are the tokens cu_seqlens[b] .. cu_seqlens[b+1]-1 of q and out
+ * (NULL: one each, token b; n_tokens == n_seqs).  A new token attends to the
+ * whole context and, with tree_mask NULL, to the new tokens up to itself: one
+ * token is a decoding step, several are a piece of a prompt or a chain of
+ * drafts.  With tree_mask [n_tokens, mask_words] it attends to its sequence's
+ * new token j where bit j%64 of its word j/64 is set: a tree of drafts, each
+ * token's bits its ancestors and itself.  Keys behind the table's last column
+ * or on no page are absent.  Everything else as v7g_attention_prefill. */
+int v7g_attention_tree(float *out, long long out_stride, const float *q, long long q_stride,
+                       const v7g_kv_pages *pages, const int32_t *block_table, int table_width,
+                       const int32_t *context_lens, const int32_t *cu_seqlens, const int64_t *tree_mask,
+                       int mask_words, int n_seqs, int n_tokens, int n_q_heads, float scale, void *workspace,
+                       int64_t workspace_bytes);
+int64_t v7g_attention_tree_workspace(int n_seqs, int n_tokens, int table_width, int page_size, int n_q_heads,
+                                     int n_kv_heads, int head_dim);
+
 #ifdef __cplusplus
 }
 #endif

@@ -70,6 +70,11 @@ SIGNATURES = {
     "v7g_swiglu_q8": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i]),
     "v7g_quantize_q8": (_i, [_vp, _vp, _vp, _i, _i, _i]),
     "v7g_embedding_gather_q8": (_i, [_vp, _vp, _i, _vp, _vp, _i, _i]),
+    "v7g_attention_prefill": (_i, [_vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp,
+                                   _ll]),
+    "v7g_attention_prefill_workspace": (_ll, [_i, _i, _i, _i, _i, _i]),
+    "v7g_attention_tree": (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _f, _vp, _ll]),
+    "v7g_attention_tree_workspace": (_ll, [_i, _i, _i, _i, _i, _i, _i]),
 }
 
 # ms_abi drop-in entries (reference names; not callable through ctypes on Linux).
@@ -101,6 +106,12 @@ class QkvStage(ctypes.Structure):
     _fields_ = [("q", QkvSide), ("k", QkvSide), ("v", QkvSide), ("n_tokens", _i), ("head_dim", _i),
                 ("cos_table", _vp), ("sin_table", _vp), ("positions", _vp), ("pos0", _i), ("rope_max_dim", _i),
                 ("table_rows", _i), ("eps", _f)]
+
+class KvPages(ctypes.Structure):
+    """v7g_kv_pages (include/v7g_lib.h)."""
+    _fields_ = [("k", _vp), ("v", _vp), ("n_layers", _i), ("n_pages", _i), ("page_size", _i), ("n_kv_heads", _i),
+                ("head_dim", _i), ("layer_stride", _ll), ("page_stride", _ll), ("token_stride", _ll)]
+
 
 _lib = None
 

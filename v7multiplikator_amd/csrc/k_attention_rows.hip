@@ -1,0 +1,468 @@
+// k_attention_rows.hip -- attention of a few rows over a long run of keys, gfx950: the tokens of a decoding step or
+// of a tree of drafts over the paged cache, and any head_dim the matrix tiles of the prompt kernel do not cover.
+//
+// out = sum_j softmax_j(q . k_j * scale) v_j with an online softmax: one pass over K and V, a running reference and
+// sum per row.  Such a call is bound by reading K and V once from HBM: a workgroup takes 16 rows (the query heads of
+// one KV head, times the tokens) and a piece of the keys; its four waves take blocks of 32 keys in turn, each with
+// its own softmax, and meet once at the end.  No wave waits for another inside the loop, and no LDS stands between
+// the loads and the matrix instructions:
+//   S^T = K Q^T: A operand (16 keys x 32 dims), lane (g = lane/16, c = lane%16) holds key c's dims 8g..8g+7, 16 bytes
+//     of a K row straight from memory.  The result leaves lane (g, c) the scores of row c at keys 4g..4g+3.
+//   O^T = V^T P^T over 32 keys: the two S tiles already are the B operand if contraction index 8g+j means key 4g+j of
+//     the first tile (j < 4) or 4g+j-4 of the second.  Lane (g, c) loads a slice of its 8 keys' V rows (16 bytes at
+//     head_dim 128: 16 lanes read 256 bytes of a row); the row index c of tile t then stands for element 8c+t, and
+//     the A operand of every tile comes from the lane's own registers with one v_perm per pair of keys.
+#include <utility>
+
+#include "v7g_attention.h"
+#include "v7g_internal.h"
+
+namespace v7g {
+
+namespace {
+
+// A head's dims in slices of 128, then 64, then 32: a lane holds 8, 4 or 2 consecutive elements of a slice of each of
+// its 8 keys, and the slice makes as many 16-row tiles.  Tile t of the slice at `base`: row index r is element
+// base + r * WIDTH + t.
+template <int D>
+struct VSlices {
+  static constexpr int n128 = D / 128, has64 = (D % 128) / 64, has32 = (D % 64) / 32;
+  static constexpr int count = n128 + has64 + has32;
+  static constexpr int width(int i) { return i < n128 ? 8 : (has64 && i == n128 ? 4 : 2); }
+  static constexpr int base(int i) { return i <= n128 ? i * 128 : n128 * 128 + 64; }
+  static constexpr int tile(int i) { return base(i) / 16; }
+};
+
+template <int WIDTH>
+__device__ __forceinline__ void load_slice(const uint16_t *p, uint32_t (&v)[4]) {
+  if constexpr (WIDTH == 8) {
+    const v4u x = *reinterpret_cast<const v4u_a8 *>(p);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+  } else if constexpr (WIDTH == 4) {
+    const v2u x = *reinterpret_cast<const v2u_a4 *>(p);
+    v[0] = x.x, v[1] = x.y;
+  } else {
+    v[0] = *reinterpret_cast<const uint32_t *>(p);
+  }
+}
+
+__device__ __forceinline__ bool nonfinite16(uint32_t x) {
+  return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u;
+}
+
+// A operand of tile t of a slice: the pairs of keys at element t.
+__device__ __forceinline__ v4u v_tile(const uint32_t (&v)[8][4], int t) {
+  const unsigned sel = (t & 1) ? 0x07060302u : 0x05040100u;
+  v4u f;
+#pragma unroll
+  for (int jj = 0; jj < 4; ++jj) f[jj] = __builtin_amdgcn_perm(v[2 * jj + 1][t / 2], v[2 * jj][t / 2], sel);
+  return f;
+}
+
+template <int... I, class F>
+__device__ __forceinline__ void each(std::integer_sequence<int, I...>, F f) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+
+template <int D, bool PAGED>
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(AttnArgs a) {
+  using S = VSlices<D>;
+  constexpr int KS = D / 32, NT = D / 16;
+  constexpr bool QREG = D <= 128;   // q in registers; wider heads read it from LDS, which all four waves share
+  constexpr bool AHEAD = D <= 256;  // the next block's K and V rows are loaded while this one is computed
+  constexpr auto slices = std::make_integer_sequence<int, S::count>{};
+  extern __shared__ float lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int g = lane >> 4, c = lane & 15;
+  const int hk = blockIdx.x % a.n_kv_heads;
+  int unit = blockIdx.x / a.n_kv_heads;
+  AttnUnit u;
+  if (!attn_find<PAGED>(a, 16, unit, -1, 0, u)) return;
+  const AttnSeq s = u.s;
+  const int rows = s.nq * a.group, row0 = u.tile * 16;
+  const int n_rows = rows - row0 < 16 ? rows - row0 : 16;
+  // this lane's row; the tile's rows behind the last one compute what that one does and are not stored
+  const int row = row0 + (c < n_rows ? c : n_rows - 1);
+  const int tok = row / a.group, head = hk * a.group + row % a.group;
+  const bool tree = PAGED && a.mask_words;
+  const int64_t *words = a.mask + (long long)(s.q0 + tok) * a.mask_words;
+  // keys below lim are seen by the row, keys from lim on by the mask's bits or not at all
+  const int lim = tree ? min(s.off, s.kv) : clampi(s.off + tok + 1, 0, s.kv);
+  const int lim_min = tree ? lim : clampi(s.off + row0 / a.group + 1, 0, s.kv);
+  const int lim_max = tree ? s.kv : clampi(s.off + (row0 + n_rows - 1) / a.group + 1, 0, s.kv);
+  const int key_lo = u.piece ? u.piece * u.piece_keys : 0;
+  const int key_hi = u.piece + 1 < u.pieces ? min((u.piece + 1) * u.piece_keys, lim_max) : lim_max;
+  const int full_hi = min(key_hi, lim_min);  // up to here every row sees every key
+
+  // ---- q rows, scaled by a power of two and split in two binary16 parts
+  v8h qh[QREG ? KS : 1], ql[QREG ? KS : 1];
+  v8h *qlds = reinterpret_cast<v8h *>(lds);  // [KS][2][64]
+  float factor;
+  {
+    const float *qr = a.q + (long long)(s.q0 + tok) * a.q_stride + (long long)head * D + g * 8;
+    float mx = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, __builtin_fabsf(qr[ks * 32 + i]));
+    mx = fmaxf(mx, xor_f(mx, 16));
+    mx = fmaxf(mx, xor_f(mx, 32));
+    const int e = q_row_exponent(mx);
+    factor = __builtin_ldexpf(a.scale_log2, -e);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = __builtin_ldexpf(qr[ks * 32 + i], e);
+      v8h hi, lo;
+      split8(x, hi, lo);
+      if constexpr (QREG) {
+        qh[ks] = hi, ql[ks] = lo;
+      } else if (wave == 0) {
+        qlds[(ks * 2) * 64 + lane] = hi;
+        qlds[(ks * 2 + 1) * 64 + lane] = lo;
+      }
+    }
+    if constexpr (!QREG) __syncthreads();
+  }
+
+  v4f acc[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) acc[t] = v4f{0, 0, 0, 0};
+  float m = -__builtin_inff(), l = 0.0f;
+
+  const uint16_t *kbase = a.k + (long long)hk * D, *vbase = a.v + (long long)hk * D;
+  // A block's two halves of 16 keys lie within one page each (pages hold a multiple of 16 tokens).
+  struct Block {
+    const uint16_t *k[2], *v[2];
+    bool ok[2];
+    int last;  // the block's last key of this piece; rows behind it are read there and masked
+  };
+  auto block_at = [&](int kb) {
+    Block b;
+    b.last = min(key_hi - 1 - kb, 31);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key0 = h && b.last < 16 ? kb : kb + 16 * h;
+      b.ok[h] = true;
+      if constexpr (PAGED) {
+        int page = a.table[(long long)u.seq * a.table_width + (key0 >> a.page_shift)];
+        page = __builtin_amdgcn_readfirstlane(page);
+        b.ok[h] = (unsigned)page < (unsigned)a.n_pages;  // a page outside the pool: its keys are absent
+        if (!b.ok[h]) page = 0;
+        const int in = key0 & ((1 << a.page_shift) - 1);
+        b.k[h] = kbase + page * a.page_stride + in * a.k_stride;
+        b.v[h] = vbase + page * a.page_stride + in * a.v_stride;
+      } else {
+        b.k[h] = kbase + (long long)(s.kv0 + key0) * a.k_stride;
+        b.v[h] = vbase + (long long)(s.kv0 + key0) * a.v_stride;
+      }
+    }
+    return b;
+  };
+  auto half_last = [&](const Block &b, int h) { return h && b.last >= 16 ? b.last - 16 : min(b.last, 15); };
+
+  v4u kr[2][KS];
+  auto load_k = [&](const Block &b) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint16_t *r = b.k[h] + (long long)min(c, half_last(b, h)) * a.k_stride + g * 8;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) kr[h][ks] = *reinterpret_cast<const v4u_a8 *>(r + ks * 32);
+    }
+  };
+  uint32_t vr[AHEAD ? S::count : 1][8][4];
+  auto load_v = [&](const Block &b, auto i, uint32_t (&v)[8][4]) {
+    constexpr int W = S::width(i);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint16_t *r = b.v[j >> 2] + (long long)min(4 * g + (j & 3), half_last(b, j >> 2)) * a.v_stride;
+      load_slice<W>(r + S::base(i) + c * W, v[j]);
+    }
+  };
+  auto scores = [&](v4f (&sc)[2]) {
+    sc[0] = sc[1] = v4f{0, 0, 0, 0};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const v8h hi = QREG ? qh[QREG ? ks : 0] : qlds[(ks * 2) * 64 + lane];
+      const v8h lo = QREG ? ql[QREG ? ks : 0] : qlds[(ks * 2 + 1) * 64 + lane];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const v8h k8 = __builtin_bit_cast(v8h, kr[h][ks]);
+        sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, hi, sc[h], 0, 0, 0);
+        sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, lo, sc[h], 0, 0, 0);
+      }
+    }
+  };
+  v8h ph, pl;
+  // The block's weights from its scores (log2 domain; -inf where a key is not seen).
+  auto weigh = [&](float (&x)[8]) {
+    float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    mx = fmaxf(mx, xor_f(mx, 16));
+    mx = fmaxf(mx, xor_f(mx, 32));
+    if (__ballot(mx > m + kAttnLazy)) {
+      const float nm = fmaxf(m, mx);
+      const float alpha = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - nm);
+      m = nm;
+      l *= alpha;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[t] *= alpha;
+    }
+    const float ref = m == -__builtin_inff() ? 0.0f : m - kAttnWeightShift;
+    float p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      p[j] = __builtin_amdgcn_exp2f(x[j] - ref);
+      l += p[j];
+    }
+    split8(p, ph, pl);
+  };
+  auto add_slice = [&](auto i, const uint32_t (&v)[8][4]) {
+#pragma unroll
+    for (int t = 0; t < S::width(i); ++t) {
+      v4f &o = acc[S::tile(i) + t];
+      const v8h v8 = __builtin_bit_cast(v8h, v_tile(v, t));
+      o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph, o, 0, 0, 0);
+      o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl, o, 0, 0, 0);
+    }
+  };
+
+  // ---- blocks whose keys every row sees
+  int kb = key_lo + wave * 32;
+  if (kb + 32 <= full_hi) {
+    Block b = block_at(kb);
+    if constexpr (AHEAD) {
+      load_k(b);
+      each(slices, [&](auto i) { load_v(b, i, vr[i]); });
+    }
+    while (true) {
+      if constexpr (!AHEAD) load_k(b);
+      v4f sc[2];
+      scores(sc);
+      const bool more = kb + 128 + 32 <= full_hi;
+      Block nb = b;
+      if (more) {
+        nb = block_at(kb + 128);
+        if constexpr (AHEAD) load_k(nb);
+      }
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = sc[j >> 2][j & 3] * factor;
+      if constexpr (PAGED)
+        if (!b.ok[0] || !b.ok[1]) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (!b.ok[j >> 2]) x[j] = -__builtin_inff();
+        }
+      weigh(x);
+      each(slices, [&](auto i) {
+        auto &v = vr[AHEAD ? i : 0];
+        if constexpr (!AHEAD) load_v(b, i, v);
+        if constexpr (PAGED)
+          if (!b.ok[0] || !b.ok[1]) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+              for (int d = 0; d < 4; ++d)
+                if (!b.ok[j >> 2]) v[j][d] = 0;
+          }
+        add_slice(i, v);
+        if constexpr (AHEAD)
+          if (more) load_v(nb, i, v);
+      });
+      kb += 128;
+      if (!more) break;
+      b = nb;
+    }
+  }
+  // ---- blocks that the mask, the piece's end or the last key cuts
+  for (; kb < key_hi; kb += 128) {
+    const Block b = block_at(kb);
+    load_k(b);
+    v4f sc[2];
+    scores(sc);
+    // which of this lane's keys a row sees, given the row's limit and token
+    auto seen_by = [&](int lim_n, const int64_t *words_n) {
+      unsigned bits = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3), d = key - s.off;
+        bool on = key < lim_n;
+        if (tree && !on) on = d < a.mask_words * 64 && ((words_n[d >> 6] >> (d & 63)) & 1);
+        if (on && key < key_hi && b.ok[j >> 2]) bits |= 1u << j;
+      }
+      return bits;
+    };
+    const unsigned seen = seen_by(lim, words);
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = (seen >> j) & 1 ? sc[j >> 2][j & 3] * factor : -__builtin_inff();
+    weigh(x);
+    // 0 * Inf would carry an infinite or NaN element of a V row to rows that do not see its key: keys that no row
+    // may read stand for zeros, and where others hold such elements the rows are taken one at a time.
+    each(slices, [&](auto i) {
+      constexpr int W = S::width(i);
+      uint32_t v[8][4];
+      load_v(b, i, v);
+      bool bad = false;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int d = 0; d < W / 2; ++d) {
+          if (kb + 16 * (j >> 2) + 4 * g + (j & 3) >= key_hi || !b.ok[j >> 2]) v[j][d] = 0;
+          bad |= nonfinite16(v[j][d]);
+        }
+      if (!__ballot(bad)) {
+        add_slice(i, v);
+        return;
+      }
+      for (int n = 0; n < 16; ++n) {
+        const int tok_n = __shfl(tok, n);
+        const unsigned seen_n = seen_by(__shfl(lim, n), a.mask + (long long)(s.q0 + tok_n) * a.mask_words);
+#pragma unroll
+        for (int t = 0; t < W; ++t) {
+          v4u f = v_tile(v, t);
+#pragma unroll
+          for (int jj = 0; jj < 4; ++jj)
+            f[jj] &= ((seen_n >> (2 * jj)) & 1 ? 0xffffu : 0u) | ((seen_n >> (2 * jj + 1)) & 1 ? 0xffff0000u : 0u);
+          const v8h v8 = __builtin_bit_cast(v8h, f);
+          const v4f z = {0, 0, 0, 0};
+          const v4f r = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph, acc[S::tile(i) + t], 0, 0, 0);
+          // a zero lo part times an infinite element is no result: hi's product decides there
+          const v4f r2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl, z, 0, 0, 0);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (c == n) acc[S::tile(i) + t][k] = __builtin_fabsf(r2[k]) < __builtin_inff() ? r[k] + r2[k] : r[k];
+        }
+      }
+    });
+  }
+
+  // ---- the four waves' results meet: 2 and 3 into 0 and 1, then 1 into 0
+  l += xor_f(l, 16);
+  l += xor_f(l, 32);
+  if constexpr (!QREG) __syncthreads();  // q in LDS is read no more
+  float *ml = lds + 2 * NT * 64 * 4;     // [2][2][64] behind the two waves' accumulators
+  v4f *ov = reinterpret_cast<v4f *>(lds);
+#pragma unroll
+  for (int step = 2; step >= 1; step >>= 1) {
+    if (wave >= step && wave < 2 * step) {
+      const int w = wave - step;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) ov[(w * NT + t) * 64 + lane] = acc[t];
+      ml[(w * 2) * 64 + lane] = m;
+      ml[(w * 2 + 1) * 64 + lane] = l;
+    }
+    __syncthreads();
+    if (wave < step) {
+      const float m2 = ml[(wave * 2) * 64 + lane], l2 = ml[(wave * 2 + 1) * 64 + lane];
+      const float nm = fmaxf(m, m2);
+      const float a1 = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - nm);
+      const float a2 = m2 == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m2 - nm);
+      l = l * a1 + l2 * a2;
+      m = nm;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[t] = acc[t] * a1 + ov[(wave * NT + t) * 64 + lane] * a2;
+    }
+    __syncthreads();
+  }
+  if (wave != 0 || c >= n_rows) return;
+  float *dst;
+  float mul;
+  if (u.pieces == 1) {
+    dst = a.out + (long long)(s.q0 + tok) * a.out_stride + (long long)head * D;
+    mul = l == 0.0f ? 0.0f : 1.0f / l;  // a row that sees nothing gives zeros
+  } else {
+    const long long slot = ((long long)unit * a.n_kv_heads + hk) * 16 + c;
+    dst = a.part_o + slot * D;
+    mul = 1.0f;
+    if (g == 0) {
+      a.part_ml[slot * 2] = m;
+      a.part_ml[slot * 2 + 1] = l;
+    }
+  }
+  each(slices, [&](auto i) {
+    constexpr int W = S::width(i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int t = 0; t < W; ++t) dst[S::base(i) + (g * 4 + k) * W + t] = acc[S::tile(i) + t][k] * mul;
+  });
+}
+
+// Joins the pieces of the rows whose keys were cut: one wave per (token, query head).
+template <bool PAGED>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, int head_dim, int tile_rows) {
+  const int lane = threadIdx.x & 63;
+  const int heads = a.n_kv_heads * a.group;
+  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (w >= (long long)a.n_tokens * heads) return;
+  const int tok = (int)(w / heads), head = (int)(w % heads);
+  const int hk = head / a.group, hr = head % a.group;
+  int unit = 0;
+  AttnUnit u;
+  if (!attn_find<PAGED>(a, tile_rows, unit, tok, hr, u) || u.pieces == 1) return;
+  const int r = (int)(((long long)(tok - u.s.q0) * a.group + hr) % tile_rows);
+  auto slot = [&](int p) { return (((long long)unit + p) * a.n_kv_heads + hk) * tile_rows + r; };
+  float m = -__builtin_inff();
+  for (int p = lane; p < u.pieces; p += 64) m = fmaxf(m, a.part_ml[slot(p) * 2]);
+  for (int x = 32; x; x >>= 1) m = fmaxf(m, xor_f(m, x));
+  const float ref = m == -__builtin_inff() ? 0.0f : m;
+  float l = 0.0f;
+  float o[8] = {0, 0, 0, 0, 0, 0, 0, 0};  // head_dim <= 512
+  for (int p = 0; p < u.pieces; ++p) {
+    const long long sl = slot(p);
+    const float wgt = __builtin_amdgcn_exp2f(a.part_ml[sl * 2] - ref);  // an empty piece: 2^-inf = 0
+    l += wgt * a.part_ml[sl * 2 + 1];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (lane + 64 * i < head_dim) o[i] += wgt * a.part_o[sl * head_dim + lane + 64 * i];
+  }
+  const float mul = l == 0.0f ? 0.0f : 1.0f / l;
+  float *dst = a.out + (long long)tok * a.out_stride + (long long)head * head_dim;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (lane + 64 * i < head_dim) dst[lane + 64 * i] = o[i] * mul;
+}
+
+template <int D>
+void rows_launch(const AttnArgs &a, bool paged, unsigned grid, hipStream_t stream) {
+  const unsigned lds = (2 * (D / 16) * 64 * 4 + 4 * 64) * 4;  // two waves' accumulators and softmax states; >= q's parts
+  if (paged)
+    enqueue(attention_rows_kernel<D, true>, dim3(grid), dim3(256), lds, stream, a);
+  else
+    enqueue(attention_rows_kernel<D, false>, dim3(grid), dim3(256), lds, stream, a);
+}
+
+}  // namespace
+
+void launch_attention(const AttnArgs &a, int head_dim, bool paged, long long units, bool split, hipStream_t stream) {
+  const unsigned grid = (unsigned)(units * a.n_kv_heads);
+  switch (head_dim) {
+    case 64: rows_launch<64>(a, paged, grid, stream); break;
+    case 96: rows_launch<96>(a, paged, grid, stream); break;
+    case 128: rows_launch<128>(a, paged, grid, stream); break;
+    case 160: rows_launch<160>(a, paged, grid, stream); break;
+    case 192: rows_launch<192>(a, paged, grid, stream); break;
+    case 224: rows_launch<224>(a, paged, grid, stream); break;
+    case 256: rows_launch<256>(a, paged, grid, stream); break;
+    case 288: rows_launch<288>(a, paged, grid, stream); break;
+    case 320: rows_launch<320>(a, paged, grid, stream); break;
+    case 352: rows_launch<352>(a, paged, grid, stream); break;
+    case 384: rows_launch<384>(a, paged, grid, stream); break;
+    case 416: rows_launch<416>(a, paged, grid, stream); break;
+    case 448: rows_launch<448>(a, paged, grid, stream); break;
+    case 480: rows_launch<480>(a, paged, grid, stream); break;
+    case 512: rows_launch<512>(a, paged, grid, stream); break;
+  }
+  if (split) {
+    const long long waves = (long long)a.n_tokens * a.n_kv_heads * a.group;
+    const unsigned blocks = (unsigned)((waves + 3) / 4);
+    if (paged)
+      enqueue(attention_join_kernel<true>, dim3(blocks), dim3(256), 0, stream, a, head_dim, 16);
+    else
+      enqueue(attention_join_kernel<false>, dim3(blocks), dim3(256), 0, stream, a, head_dim, 16);
+  }
+}
+
+}  // namespace v7g

@@ -18,6 +18,7 @@
 #include <vector>
 
 #include "v7g_alias.h"
+#include "v7g_attention.h"
 #include "v7g_rope_tables.h"
 #include "v7g_internal.h"
 #include "../../include/v7g_lib.h"
@@ -934,6 +935,177 @@ V7_ABI void v7s_rope_init(int head_dim, float rope_base) {
     v7g_rope_init_llama3(head_dim, c.base, kRopeMaxPositions, c.factor, c.low, c.high, c.orig_max_pos);
   else
     v7g_rope_init(head_dim, c.base, kRopeMaxPositions);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- attention
+
+namespace {
+
+// How a call is cut: tiles of kAttnRowTile rows, and pieces of their keys where the tiles alone leave compute units
+// idle.  max_keys is the most keys a sequence can have, as far as the host knows.
+struct AttnPlan {
+  int target = 0;         // units per KV head aimed at, 0: whole tiles
+  long long units = 0;    // at most, per KV head
+  long long workspace = 0;
+};
+
+AttnPlan attn_plan(int n_seqs, int n_tokens, int group, int n_kv_heads, int head_dim, long long max_keys) {
+  AttnPlan p;
+  const long long tiles = (long long)n_tokens * group / v7g::kAttnRowTile + n_seqs;
+  p.units = tiles;
+  if (tiles * n_kv_heads < v7g::kAttnUnits && max_keys > v7g::kAttnMinChunk) {
+    p.target = (v7g::kAttnUnits + n_kv_heads - 1) / n_kv_heads;
+    p.units = tiles + p.target;
+    p.workspace = p.units * n_kv_heads * v7g::kAttnRowTile * (head_dim + 2) * 4;
+  }
+  return p;
+}
+
+int check_attention(int n_seqs, int n_tokens, int n_q_heads, int n_kv_heads, int head_dim) {
+  if (n_seqs < 0 || n_tokens < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0)
+    return V7G_ERR_SHAPE;
+  if (head_dim < 64 || head_dim > 512 || head_dim % 32 != 0) return V7G_ERR_SHAPE;
+  if ((long long)n_tokens * n_q_heads >= (1LL << 31) - 64 || n_seqs >= (1 << 30)) return V7G_ERR_SHAPE;
+  const long long tiles = (long long)n_tokens * (n_q_heads / n_kv_heads) / v7g::kAttnRowTile + n_seqs;
+  return (tiles + v7g::kAttnUnits) * n_kv_heads >= (1LL << 31) ? V7G_ERR_SHAPE : V7G_OK;
+}
+
+bool bad_stride(long long stride, long long rows, long long row_len) {
+  return stride % 4 != 0 || (rows > 1 && stride < row_len);
+}
+
+int launch_attn(v7g::AttnArgs &a, const AttnPlan &p, int head_dim, bool paged, void *workspace) {
+  a.split_target = p.target;
+  a.part_o = static_cast<float *>(workspace);
+  a.part_ml = a.part_o ? a.part_o + p.units * a.n_kv_heads * v7g::kAttnRowTile * head_dim : nullptr;
+  v7g::launch_attention(a, head_dim, paged, p.units, p.target != 0, stream());
+  return check_launch();
+}
+
+int check_pages(const v7g_kv_pages &g) {
+  if (g.n_layers <= 0 || g.n_pages < 0 || g.page_size < 16 || g.page_size > 65536 ||
+      (g.page_size & (g.page_size - 1)) || g.n_kv_heads <= 0 || g.head_dim <= 0)
+    return V7G_ERR_SHAPE;
+  const long long row = (long long)g.n_kv_heads * g.head_dim;
+  if (row % 4 || row >= (1LL << 30) || bad_stride(g.token_stride, g.page_size, row)) return V7G_ERR_SHAPE;
+  const long long page = (g.page_size - 1) * g.token_stride + row;
+  if (g.page_stride % 4 || (g.n_pages > 1 && g.page_stride < page)) return V7G_ERR_SHAPE;
+  const long long layer = (g.n_pages > 1 ? (g.n_pages - 1) * g.page_stride : 0) + page;
+  if (g.layer_stride % 4 || (g.n_layers > 1 && g.layer_stride < layer)) return V7G_ERR_SHAPE;
+  if (g.n_pages == 0) return V7G_OK;
+  if (!g.k || !g.v) return V7G_ERR_NULL;
+  return (((uintptr_t)g.k | (uintptr_t)g.v) & 7u) ? V7G_ERR_ALIGN : V7G_OK;
+}
+
+// One side's pages: page against page where all layers' pages lie at one stride, else the whole range.
+v7g::Span pages_span(const v7g_kv_pages &g, const uint16_t *p, int layers) {
+  if (g.n_pages <= 0) return v7g::flat_span(nullptr, 0);
+  const long long page = ((g.page_size - 1) * g.token_stride + (long long)g.n_kv_heads * g.head_dim) * 2;
+  if (layers == 1) return v7g::row_span(p, g.n_pages, g.page_stride * 2, page);
+  if (g.layer_stride == g.n_pages * g.page_stride)
+    return v7g::row_span(p, (long long)layers * g.n_pages, g.page_stride * 2, page);
+  return v7g::flat_span(p, ((layers - 1) * g.layer_stride + (g.n_pages - 1) * g.page_stride) * 2 + page);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t v7g_attention_prefill_workspace(int n_seqs, int n_tokens, int n_kv_tokens, int n_q_heads, int n_kv_heads,
+                                        int head_dim) {
+  if (check_attention(n_seqs, n_tokens, n_q_heads, n_kv_heads, head_dim)) return 0;
+  return attn_plan(n_seqs, n_tokens, n_q_heads / n_kv_heads, n_kv_heads, head_dim, n_kv_tokens).workspace;
+}
+
+int v7g_attention_prefill(float *out, long long out_stride, const float *q, long long q_stride, const uint16_t *k,
+                          long long k_stride, const uint16_t *v, long long v_stride, const int32_t *cu_seqlens,
+                          const int32_t *cu_seqlens_k, int n_seqs, int n_tokens, int n_kv_tokens, int n_q_heads,
+                          int n_kv_heads, int head_dim, float scale, void *workspace, int64_t workspace_bytes) {
+  if (int rc = check_attention(n_seqs, n_tokens, n_q_heads, n_kv_heads, head_dim)) return fail(rc);
+  const long long qrow = (long long)n_q_heads * head_dim, krow = (long long)n_kv_heads * head_dim;
+  if (n_kv_tokens < 0 || (!cu_seqlens_k && n_kv_tokens != n_tokens)) return fail(V7G_ERR_SHAPE);
+  if (bad_stride(out_stride, n_tokens, qrow) || bad_stride(q_stride, n_tokens, qrow) ||
+      bad_stride(k_stride, n_kv_tokens, krow) || bad_stride(v_stride, n_kv_tokens, krow))
+    return fail(V7G_ERR_SHAPE);
+  if (n_tokens == 0 || n_seqs == 0) return V7G_OK;
+  const AttnPlan p = attn_plan(n_seqs, n_tokens, n_q_heads / n_kv_heads, n_kv_heads, head_dim, n_kv_tokens);
+  if (!out || !q || !cu_seqlens || (n_kv_tokens > 0 && (!k || !v)) || (p.workspace && !workspace))
+    return fail(V7G_ERR_NULL);
+  if (workspace_bytes < p.workspace) return fail(V7G_ERR_SHAPE);
+  if (!al16(out) || !al16(q) || !al16(workspace) || (((uintptr_t)k | (uintptr_t)v) & 7u) ||
+      (((uintptr_t)cu_seqlens | (uintptr_t)cu_seqlens_k) & 3u))
+    return fail(V7G_ERR_ALIGN);
+  const v7g::Span W = v7g::flat_span(p.workspace ? workspace : nullptr, p.workspace);
+  const long long cu_bytes = 4LL * (n_seqs + 1);
+  if (int ac = check_alias({v7g::row_span(out, n_tokens, out_stride * 4, qrow * 4), W},
+                           {v7g::row_span(q, n_tokens, q_stride * 4, qrow * 4),
+                            v7g::row_span(k, n_kv_tokens, k_stride * 2, krow * 2),
+                            v7g::row_span(v, n_kv_tokens, v_stride * 2, krow * 2),
+                            v7g::flat_span(cu_seqlens, cu_bytes), v7g::flat_span(cu_seqlens_k, cu_bytes)}))
+    return fail(ac);
+  if (int pc = check_ptrs({out, q, k, v, cu_seqlens, cu_seqlens_k, p.workspace ? workspace : nullptr}))
+    return fail(pc);
+  v7g::AttnArgs a = {};
+  a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
+  a.k = k, a.v = v, a.k_stride = k_stride, a.v_stride = v_stride;
+  a.cu_q = cu_seqlens, a.cu_k = cu_seqlens_k;
+  a.n_seqs = n_seqs, a.n_tokens = n_tokens, a.n_kv = n_kv_tokens;
+  a.n_kv_heads = n_kv_heads, a.group = n_q_heads / n_kv_heads;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  return launch_attn(a, p, head_dim, false, workspace);
+}
+
+int64_t v7g_attention_tree_workspace(int n_seqs, int n_tokens, int table_width, int page_size, int n_q_heads,
+                                     int n_kv_heads, int head_dim) {
+  if (table_width < 0 || page_size < 0 || check_attention(n_seqs, n_tokens, n_q_heads, n_kv_heads, head_dim)) return 0;
+  return attn_plan(n_seqs, n_tokens, n_q_heads / n_kv_heads, n_kv_heads, head_dim, (long long)table_width * page_size)
+      .workspace;
+}
+
+int v7g_attention_tree(float *out, long long out_stride, const float *q, long long q_stride,
+                       const v7g_kv_pages *pages, const int32_t *block_table, int table_width,
+                       const int32_t *context_lens, const int32_t *cu_seqlens, const int64_t *tree_mask,
+                       int mask_words, int n_seqs, int n_tokens, int n_q_heads, float scale, void *workspace,
+                       int64_t workspace_bytes) {
+  if (!pages) return fail(V7G_ERR_NULL);
+  const v7g_kv_pages &g = *pages;
+  if (int rc = check_pages(g)) return fail(rc);
+  if (int rc = check_attention(n_seqs, n_tokens, n_q_heads, g.n_kv_heads, g.head_dim)) return fail(rc);
+  const long long qrow = (long long)n_q_heads * g.head_dim, cap = (long long)table_width * g.page_size;
+  if (table_width < 0 || cap >= (1LL << 31) - 64 || (!cu_seqlens && n_tokens != n_seqs)) return fail(V7G_ERR_SHAPE);
+  if (tree_mask ? (mask_words <= 0 || mask_words >= (1 << 24)) : mask_words != 0) return fail(V7G_ERR_SHAPE);
+  if (bad_stride(out_stride, n_tokens, qrow) || bad_stride(q_stride, n_tokens, qrow)) return fail(V7G_ERR_SHAPE);
+  if (n_tokens == 0 || n_seqs == 0) return V7G_OK;
+  const AttnPlan p = attn_plan(n_seqs, n_tokens, n_q_heads / g.n_kv_heads, g.n_kv_heads, g.head_dim, cap);
+  // with no page or no table there is no key: every token of a sequence gives zeros
+  const bool none = g.n_pages == 0 || table_width == 0;
+  if (!out || !q || !context_lens || (!none && !block_table) || (p.workspace && !workspace)) return fail(V7G_ERR_NULL);
+  if (workspace_bytes < p.workspace) return fail(V7G_ERR_SHAPE);
+  if (!al16(out) || !al16(q) || !al16(workspace) || ((uintptr_t)tree_mask & 7u) ||
+      (((uintptr_t)block_table | (uintptr_t)context_lens | (uintptr_t)cu_seqlens) & 3u))
+    return fail(V7G_ERR_ALIGN);
+  const v7g::Span W = v7g::flat_span(p.workspace ? workspace : nullptr, p.workspace);
+  if (int ac = check_alias({v7g::row_span(out, n_tokens, out_stride * 4, qrow * 4), W},
+                           {v7g::row_span(q, n_tokens, q_stride * 4, qrow * 4), pages_span(g, g.k, 1),
+                            pages_span(g, g.v, 1), v7g::flat_span(block_table, 4LL * n_seqs * table_width),
+                            v7g::flat_span(context_lens, 4LL * n_seqs), v7g::flat_span(cu_seqlens, 4LL * (n_seqs + 1)),
+                            v7g::flat_span(tree_mask, 8LL * n_tokens * mask_words)}))
+    return fail(ac);
+  if (int pc = check_ptrs({out, q, g.k, g.v, block_table, context_lens, cu_seqlens, tree_mask,
+                           p.workspace ? workspace : nullptr}))
+    return fail(pc);
+  v7g::AttnArgs a = {};
+  a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
+  a.k = g.k, a.v = g.v, a.k_stride = a.v_stride = g.token_stride, a.page_stride = g.page_stride;
+  a.table = block_table, a.table_width = none ? 0 : table_width, a.n_pages = g.n_pages;
+  a.page_shift = __builtin_ctz((unsigned)g.page_size);
+  a.ctx = context_lens, a.cu_q = cu_seqlens, a.mask = tree_mask, a.mask_words = mask_words;
+  a.n_seqs = n_seqs, a.n_tokens = n_tokens;
+  a.n_kv_heads = g.n_kv_heads, a.group = n_q_heads / g.n_kv_heads;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  return launch_attn(a, p, g.head_dim, true, workspace);
 }
 
 }  // extern "C"

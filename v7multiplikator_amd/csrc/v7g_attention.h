@@ -1,0 +1,188 @@
+// v7g_attention.h -- what the attention kernels share: their arguments, how the work is cut into units, and the
+// two-part binary16 form of f32 operands.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "v7g_device.h"
+
+namespace v7g {
+
+// One attention call.  Rows are (token, query head of the group) pairs: the G query heads that share a KV head lie
+// next to each other in a token, so row r of a sequence and KV head hk is head hk*G + r%G of its token r/G, and a
+// tile of rows reads each K/V row once for all of them.
+struct AttnArgs {
+  const float *q;
+  float *out;
+  long long q_stride, out_stride;  // f32 elements between tokens
+  const uint16_t *k, *v;           // binary16; paged: page 0
+  long long k_stride, v_stride;    // binary16 elements between tokens (paged: within a page)
+  long long page_stride;           // paged: binary16 elements between pages
+  const int32_t *table;            // paged: [n_seqs, table_width] page of each page_size tokens
+  const int32_t *ctx;              // paged: tokens in the cache before this call's
+  const int32_t *cu_q;             // [n_seqs + 1] first token of each sequence, or nullptr: token b is sequence b
+  const int32_t *cu_k;             // packed: the same of the K/V rows
+  const int64_t *mask;             // paged: per token mask_words words, bit j = attends to the sequence's new token j
+  int mask_words;                  // 0: causal
+  int table_width, page_shift, n_pages;
+  int n_seqs, n_tokens, n_kv;  // n_kv: packed K/V rows
+  int n_kv_heads, group;
+  float scale_log2;  // the score scale times log2(e)
+  int split_target;  // units per KV head aimed at; 0: no tile is split along the keys
+  float *part_o;     // [unit, KV head, tile row, head_dim]
+  float *part_ml;    // [unit, KV head, tile row, 2]: running maximum (log2 domain) and sum
+};
+
+constexpr int kAttnRowTile = 16;    // rows of a tile
+constexpr int kAttnUnits = 1024;    // units that fill the chip: four workgroups for each of 256 compute units
+constexpr int kAttnMinChunk = 256;  // keys; shorter pieces cost more in joining than they save
+
+// A sequence's tokens and keys.  Lengths and offsets come from device memory, so each is brought into the range of
+// its buffer: a wrong one gives wrong rows, never an access outside.
+struct AttnSeq {
+  int q0, nq;   // its tokens in q
+  int kv0, kv;  // its keys: packed rows kv0.., or positions 0.. of its pages
+  int off;      // position of its token 0 among the keys
+};
+
+__device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
+
+template <bool PAGED>
+__device__ __forceinline__ AttnSeq attn_seq(const AttnArgs &a, int b) {
+  AttnSeq s;
+  if (a.cu_q) {
+    s.q0 = clampi(a.cu_q[b], 0, a.n_tokens);
+    s.nq = clampi(a.cu_q[b + 1], s.q0, a.n_tokens) - s.q0;
+  } else {
+    s.q0 = b;
+    s.nq = 1;
+  }
+  if constexpr (PAGED) {
+    const int cap = a.table_width << a.page_shift;  // below 2^31 (the entry's check)
+    s.kv0 = 0;
+    s.off = clampi(a.ctx[b], 0, cap);
+    s.kv = s.nq > cap - s.off ? cap : s.off + s.nq;
+  } else {
+    if (a.cu_k) {
+      s.kv0 = clampi(a.cu_k[b], 0, a.n_kv);
+      s.kv = clampi(a.cu_k[b + 1], s.kv0, a.n_kv) - s.kv0;
+    } else {  // as many K/V rows as tokens, at the same places
+      s.kv0 = s.q0;
+      s.kv = s.nq;
+    }
+    s.off = s.kv - s.nq;  // negative: the first tokens see nothing
+  }
+  return s;
+}
+
+// A unit of work: TM rows of a sequence and one piece of its keys.
+struct AttnUnit {
+  AttnSeq s;
+  int seq, tile, piece, pieces, piece_keys;
+};
+
+__device__ __forceinline__ int lane_id() { return __lane_id(); }
+
+// Keys per piece: the summed key counts of all tiles over the units aimed at, in whole blocks of 64.  Every
+// workgroup derives the same number from the lengths, so the host needs none of them.
+template <bool PAGED>
+__device__ __forceinline__ int attn_piece_keys(const AttnArgs &a, int tile_rows) {
+  if (!a.split_target) return 0x7fffffff;
+  long long sum = 0;
+  for (int b = lane_id(); b < a.n_seqs; b += 64) {
+    const AttnSeq s = attn_seq<PAGED>(a, b);
+    sum += (long long)(((long long)s.nq * a.group + tile_rows - 1) / tile_rows) * s.kv;
+  }
+  for (int m = 32; m; m >>= 1) sum += __shfl_xor(sum, m);
+  long long keys = (sum + a.split_target - 1) / a.split_target;
+  keys = (keys + 63) & ~63ll;
+  return keys < kAttnMinChunk ? kAttnMinChunk : (keys > 0x7fffffc0 ? 0x7fffffff : (int)keys);
+}
+
+// Unit number `want` in the order of sequences, tiles and pieces; with `of_token` the unit of that token's row
+// instead (its first piece), its number returned in `want`.  False: past the last.  Every lane of the wave takes part.
+template <bool PAGED>
+__device__ __forceinline__ bool attn_find(const AttnArgs &a, int tile_rows, int &want, int of_token, int row_in_token,
+                                          AttnUnit &u) {
+  u.piece_keys = attn_piece_keys<PAGED>(a, tile_rows);
+  int base = 0;
+  for (int b0 = 0; b0 < a.n_seqs; b0 += 64) {
+    const int b = b0 + lane_id();
+    AttnSeq s{0, 0, 0, 0, 0};
+    int units = 0, pieces = 1;
+    if (b < a.n_seqs) {
+      s = attn_seq<PAGED>(a, b);
+      const int tiles = (int)(((long long)s.nq * a.group + tile_rows - 1) / tile_rows);
+      pieces = s.kv <= u.piece_keys ? 1 : (int)(((long long)s.kv + u.piece_keys - 1) / u.piece_keys);
+      units = tiles * pieces;
+    }
+    int incl = units;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(incl, d);
+      if (lane_id() >= d) incl += o;
+    }
+    const bool mine = of_token >= 0 ? (of_token >= s.q0 && of_token < s.q0 + s.nq)
+                                    : (want >= base + incl - units && want < base + incl);
+    const unsigned long long hit = __ballot(mine);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      u.seq = b0 + l;
+      u.s.q0 = __builtin_amdgcn_readlane(s.q0, l);
+      u.s.nq = __builtin_amdgcn_readlane(s.nq, l);
+      u.s.kv0 = __builtin_amdgcn_readlane(s.kv0, l);
+      u.s.kv = __builtin_amdgcn_readlane(s.kv, l);
+      u.s.off = __builtin_amdgcn_readlane(s.off, l);
+      u.pieces = __builtin_amdgcn_readlane(pieces, l);
+      const int first = base + __builtin_amdgcn_readlane(incl - units, l);
+      if (of_token >= 0) {
+        u.tile = (int)(((long long)(of_token - u.s.q0) * a.group + row_in_token) / tile_rows);
+        u.piece = 0;
+        want = first + u.tile * u.pieces;
+      } else {
+        u.tile = (want - first) / u.pieces;
+        u.piece = (want - first) - u.tile * u.pieces;
+      }
+      return true;
+    }
+    base += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return false;
+}
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef unsigned int v4u __attribute__((ext_vector_type(4)));
+typedef unsigned int v2u __attribute__((ext_vector_type(2)));
+// K/V rows are 8-byte aligned (what the K/V pack asks of them).
+typedef v4u v4u_a8 __attribute__((aligned(8)));
+typedef v2u v2u_a4 __attribute__((aligned(4)));
+typedef v4f v4f_a16 __attribute__((aligned(16)));
+
+// The f32 operands of the two products (q rows and softmax weights) enter the binary16 matrix instructions as
+// x = hi + lo with hi = f16(x) and lo = f16(x - hi): 22 bits of x, so that the products with the binary16 K and V
+// rows keep f32 accuracy; the accumulators are f32.  A q row is first scaled by the power of two that brings its
+// largest element to [2^12, 2^13): neither part overflows, and lo's subnormals start 2^-36 below the row's largest.
+__device__ __forceinline__ int q_row_exponent(float row_max) {
+  const int e = (int)((__builtin_bit_cast(uint32_t, row_max) >> 23) & 255u);
+  return (e == 0 || e == 255) ? 0 : 139 - e;
+}
+
+__device__ __forceinline__ void split8(const float (&x)[8], v8h &hi, v8h &lo) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    hi[i] = (_Float16)x[i];
+    lo[i] = (_Float16)(x[i] - (float)hi[i]);
+  }
+}
+
+// Softmax weights are 2^(score - reference + 4): the reference follows the running maximum only when a score
+// passes it by more than 8, so weights reach 2^12 at most and lo keeps its bits for weights near 1.
+constexpr float kAttnWeightShift = 4.0f;
+constexpr float kAttnLazy = 8.0f;
+
+// Shapes and pointers are validated by the caller; units: at most, per KV head; split: pieces have to be joined.
+void launch_attention(const AttnArgs &a, int head_dim, bool paged, long long units, bool split, hipStream_t stream);
+
+}  // namespace v7g

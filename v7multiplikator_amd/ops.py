@@ -28,6 +28,7 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
+import math
 import os
 import sys
 
@@ -558,3 +559,143 @@ def rope_tables(n_pos: int, head_dim: int, rope_base: float, device="cuda", llam
                                             int(llama3["original_max_position_embeddings"]))
     _lib.check(rc, "rope_tables")
     return c, s
+
+
+# ---------------------------------------------------------------- around the K/V cache
+
+def _workspace(n: int, device):
+    """Scratch of one call from torch's allocator: ordered on the stream the call runs on, and a captured graph's own."""
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _scale(scale, head_dim):
+    return 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+
+
+def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                      cu_seqlens_k: torch.Tensor | None = None, scale: float | None = None,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention over packed sequences with grouped heads, out = softmax(q k^T * scale) v in f32.
+
+    q [T, Hq, D] f32 and k, v [S, Hk, D] float16 (heads of a token contiguous, token strides free).  Sequence b has
+    the tokens cu_seqlens[b] .. cu_seqlens[b+1]-1 of q and the rows cu_seqlens_k[b] .. of k and v (int32 on the
+    device; None: the same as cu_seqlens); its token i of n sees its first i + 1 + m - n rows of m.  scale defaults
+    to 1/sqrt(D).  A token that sees nothing gives zeros; tokens of out behind the last sequence are left as they
+    were."""
+    _need(q, torch.float32, "q", contiguous=False)
+    T, Hq, D, qs = _heads_view(q, "q")
+    for t, n in ((k, "k"), (v, "v")):
+        _need(t, torch.float16, n, contiguous=False)
+    S, Hk, Dk, ks = _heads_view(k, "k")
+    Sv, Hv, Dv, vs = _heads_view(v, "v")
+    if (Sv, Hv, Dv) != (S, Hk, Dk) or Dk != D:
+        raise ValueError("k and v must both be [kv_tokens, kv_heads, head_dim] with q's head_dim")
+    _need(cu_seqlens, torch.int32, "cu_seqlens")
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+        raise ValueError("cu_seqlens must hold n_seqs + 1 offsets")
+    if cu_seqlens_k is not None:
+        _need(cu_seqlens_k, torch.int32, "cu_seqlens_k")
+        if cu_seqlens_k.shape != cu_seqlens.shape:
+            raise ValueError("cu_seqlens_k must match cu_seqlens")
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=torch.float32, device=q.device)
+    _need(out, torch.float32, "out", contiguous=False)
+    To, Ho, Do, os_ = _heads_view(out, "out")
+    if (To, Ho, Do) != (T, Hq, D):
+        raise ValueError("out must match q")
+    L = _lib.load()
+    n_seqs = cu_seqlens.numel() - 1
+    ws = _workspace(L.v7g_attention_prefill_workspace(n_seqs, T, S, Hq, Hk, D), q.device)
+    _bind(q)
+    rc = L.v7g_attention_prefill(out.data_ptr(), os_, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+                                 cu_seqlens.data_ptr(), _ptr(cu_seqlens_k), n_seqs, T, S, Hq, Hk, D,
+                                 _scale(scale, D), _ptr(ws), 0 if ws is None else ws.numel())
+    _lib.check(rc, "attention_prefill")
+    return out
+
+
+def _kv_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, layered: bool) -> _lib.KvPages:
+    """v7g_kv_pages of the pages [n_pages, page_size, Hk, D] of one layer, or with `layered` also
+    [layers, n_pages, page_size, Hk, D]; the K and V pages share their strides."""
+    for t, n in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        _need(t, torch.float16, n, contiguous=False)
+    if k_pages.dim() != 4 and not (layered and k_pages.dim() == 5):
+        raise ValueError("k_pages must be [n_pages, page_size, kv_heads, head_dim]" +
+                         (" or [layers, ...]" if layered else ""))
+    if v_pages.shape != k_pages.shape or v_pages.stride() != k_pages.stride():
+        raise ValueError("v_pages must have the shape and strides of k_pages")
+    P, ps, H, D = k_pages.shape[-4:]
+    st = k_pages.stride()
+    if st[-1] != 1 or (H > 1 and st[-2] != D):
+        raise ValueError("heads of one token must be contiguous in the pages")
+    g = _lib.KvPages()
+    g.k, g.v = k_pages.data_ptr() or None, v_pages.data_ptr() or None
+    g.n_layers, g.layer_stride = (k_pages.shape[0], st[0]) if k_pages.dim() == 5 else (1, 0)
+    g.n_pages, g.page_size, g.n_kv_heads, g.head_dim = P, ps, H, D
+    g.page_stride, g.token_stride = st[-4], st[-3]
+    return g
+
+
+def _table(block_table, rows, name="block_table"):
+    _need(block_table, torch.int32, name)
+    if block_table.dim() != 2 or (rows is not None and block_table.shape[0] != rows):
+        raise ValueError(f"{name} must be [sequences, pages per sequence]")
+
+
+def _rows_i32(t, rows, name):
+    _need(t, torch.int32, name)
+    if t.dim() != 1 or t.numel() != rows:
+        raise ValueError(f"{name} must hold {rows} int32")
+
+
+def attention_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                   context_lens: torch.Tensor, cu_seqlens: torch.Tensor | None = None,
+                   tree_mask: torch.Tensor | None = None, scale: float | None = None,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of new tokens over a paged binary16 cache: a decoding step, or a tree of drafts.
+
+    q [T, Hq, D] f32; k_pages, v_pages [n_pages, page_size, Hk, D] float16; block_table [B, W] and context_lens [B]
+    int32.  Sequence b's pages hold context_lens[b] tokens and behind them its new tokens, whose q rows are
+    cu_seqlens[b] .. cu_seqlens[b+1]-1 (None: one each, T == B).  A new token sees the context and the new tokens up
+    to itself, or, with tree_mask (int64, [T] or [T, words]), the new tokens j of its sequence whose bit j%64 of word
+    j/64 is set.  Everything else as attention_prefill."""
+    _need(q, torch.float32, "q", contiguous=False)
+    T, Hq, D, qs = _heads_view(q, "q")
+    g = _kv_pages(k_pages, v_pages, False)
+    if g.head_dim != D:
+        raise ValueError("the pages must have q's head_dim")
+    _need(context_lens, torch.int32, "context_lens")
+    B = context_lens.numel()
+    _rows_i32(context_lens, B, "context_lens")
+    _table(block_table, B)
+    if cu_seqlens is not None:
+        _rows_i32(cu_seqlens, B + 1, "cu_seqlens")
+    elif T != B:
+        raise ValueError("without cu_seqlens there is one token per sequence")
+    words = 0
+    if tree_mask is not None:
+        _need(tree_mask, torch.int64, "tree_mask")
+        if tree_mask.dim() not in (1, 2) or tree_mask.shape[0] != T:
+            raise ValueError("tree_mask must be [tokens] or [tokens, words]")
+        words = tree_mask.shape[1] if tree_mask.dim() == 2 else 1
+        if words == 0:
+            raise ValueError("tree_mask must hold at least one word per token")
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=torch.float32, device=q.device)
+    _need(out, torch.float32, "out", contiguous=False)
+    To, Ho, Do, os_ = _heads_view(out, "out")
+    if (To, Ho, Do) != (T, Hq, D):
+        raise ValueError("out must match q")
+    L = _lib.load()
+    W = block_table.shape[1]
+    ws = _workspace(L.v7g_attention_tree_workspace(B, T, W, g.page_size, Hq, g.n_kv_heads, D), q.device)
+    _bind(q)
+    rc = L.v7g_attention_tree(out.data_ptr(), os_, q.data_ptr(), qs, ctypes.addressof(g), block_table.data_ptr(), W,
+                              context_lens.data_ptr(), _ptr(cu_seqlens), _ptr(tree_mask) if T else None,
+                              words if T else 0, B, T, Hq, _scale(scale, D), _ptr(ws), 0 if ws is None else ws.numel())
+    _lib.check(rc, "attention_tree")
+    return out
