@@ -513,6 +513,67 @@ int v7g_attention_tree(float *out, long long out_stride, const float *q, long lo
 int64_t v7g_attention_tree_workspace(int n_seqs, int n_tokens, int table_width, int page_size, int n_q_heads,
                                      int n_kv_heads, int head_dim);
 
+/* The K and V rows of n_tokens tokens, f32, rounded to nearest even into the
+ * pages (layer 0): v7g_kv_pack_f16_kv whose destination is a place in the
+ * cache.  Token t's rows of n_kv_heads * head_dim floats at k_src +
+ * t*src_stride and v_src + t*src_stride go to position positions[t] of the
+ * sequence of block table row seqs[t] (NULL: row t; n_tokens <= n_seqs).  A
+ * token with no such row, position or page is skipped.  The places of one call
+ * are distinct, and on pages that no other sequence shares.  src 16-byte
+ * aligned, src_stride % 4 == 0. */
+int v7g_kv_pack_f16_pages(const v7g_kv_pages *pages, const float *k_src, const float *v_src, long long src_stride,
+                          const int32_t *block_table, int table_width, int n_seqs, const int32_t *positions,
+                          const int32_t *seqs, int n_tokens);
+
+/* Sequences forked, freed and grown, all n_seqs rows of a block table at once:
+ * row r of table_out becomes the sequence of row parents[r] of block_table (r:
+ * it stays; another row: a fork; outside [0, n_seqs): row r is freed), with
+ * room for reserve[r] more tokens (NULL: none).  lens [n_seqs] are the tokens
+ * of the sequences; a row holds its leading entries that name a page, and no
+ * more than lens tokens on them.  refs [n_pages] counts the rows and other
+ * holders of each page; a page whose count is 0 is free.
+ *   - The full pages are shared: the fork's row names its parent's.
+ *   - The last, partly filled page belongs to one row: the parent's own if
+ *     that stays, else the lowest fork, which also take over pages behind it.
+ *     Every other fork gets a page of its own with those tokens copied, in
+ *     every layer, K and V.
+ *   - New pages (for copies, then for reserved tokens, up to table_width) are
+ *     the lowest free ones, counted after this call's releases, in the order
+ *     of rows and then of places.  If they run out, the requests left over are
+ *     counted in short_out[0]: their entries stay -1, and a fork without its
+ *     copy ends with its full pages (lens_out).
+ * table_out, lens_out, refs_out [n_pages] and short_out [1] are apart from the
+ * inputs.  Entries behind a row's pages are -1.  workspace:
+ * v7g_kv_pages_assign_workspace(n_seqs, n_pages) bytes, as for the attention. */
+int v7g_kv_pages_assign(const v7g_kv_pages *pages, int32_t *table_out, int32_t *lens_out, int32_t *refs_out,
+                        int32_t *short_out, const int32_t *block_table, const int32_t *lens, const int32_t *refs,
+                        const int32_t *parents, const int32_t *reserve, int n_seqs, int table_width, void *workspace,
+                        int64_t workspace_bytes);
+int64_t v7g_kv_pages_assign_workspace(int n_seqs, int n_pages);
+
+/* Accepted drafts: of the new tokens behind lens[r] tokens of block table row
+ * r, those numbered path[r][0..n_path[r]-1] (strictly ascending, as a path
+ * through a tree whose tokens follow their ancestors is) move to the places
+ * lens[r], lens[r] + 1, ..., in every layer, K and V; lens_out[r] = lens[r] +
+ * their number.  The path ends at its first entry that does not ascend or has
+ * no page.  path [n_seqs, path_width]; lens_out apart from the inputs.  The
+ * rows' pages from lens[r] on are shared with no other row. */
+int v7g_kv_pages_compact(const v7g_kv_pages *pages, int32_t *lens_out, const int32_t *block_table, int table_width,
+                         const int32_t *lens, const int32_t *path, int path_width, const int32_t *n_path, int n_seqs);
+
+/* Scores of n_tokens logit rows of vocab floats (row t at logits + t*stride):
+ * logprob[t] of token ids[t] (NaN for an id outside the vocabulary), the
+ * entropy of the row in nats, and its top_k most likely tokens in order with
+ * their log probabilities, [n_tokens, top_k] (0 <= top_k <= 64, top_k <=
+ * vocab; equal logits: the lower index first; NaN counts as the largest).
+ * Logits of -inf have probability 0; a row that holds NaN or +inf, or nothing
+ * above -inf, has NaN for every probability.  workspace:
+ * v7g_token_logprobs_workspace(...) bytes, as for the attention. */
+int v7g_token_logprobs(float *logprob, float *entropy, float *top_logprob, int32_t *top_ids, const float *logits,
+                       long long stride, const int32_t *ids, int n_tokens, int vocab, int top_k, void *workspace,
+                       int64_t workspace_bytes);
+int64_t v7g_token_logprobs_workspace(int n_tokens, int vocab, int top_k);
+
 #ifdef __cplusplus
 }
 #endif

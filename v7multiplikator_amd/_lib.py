@@ -75,6 +75,12 @@ SIGNATURES = {
     "v7g_attention_prefill_workspace": (_ll, [_i, _i, _i, _i, _i, _i]),
     "v7g_attention_tree": (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _f, _vp, _ll]),
     "v7g_attention_tree_workspace": (_ll, [_i, _i, _i, _i, _i, _i, _i]),
+    "v7g_kv_pack_f16_pages": (_i, [_vp, _vp, _vp, _ll, _vp, _i, _i, _vp, _vp, _i]),
+    "v7g_kv_pages_assign": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _ll]),
+    "v7g_kv_pages_assign_workspace": (_ll, [_i, _i]),
+    "v7g_kv_pages_compact": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _i]),
+    "v7g_token_logprobs": (_i, [_vp, _vp, _vp, _vp, _vp, _ll, _vp, _i, _i, _i, _vp, _ll]),
+    "v7g_token_logprobs_workspace": (_ll, [_i, _i, _i]),
 }
 
 # ms_abi drop-in entries (reference names; not callable through ctypes on Linux).

@@ -1,0 +1,299 @@
+// k_logprobs.hip -- log probabilities of given tokens, entropy and the most likely tokens of logit rows, gfx950.
+//
+//   logprob = x_id - m - log s,  entropy = log s - w / s,  s = sum e^(x-m), w = sum e^(x-m) (x-m),  m = max x
+//
+// One pass over the logits, which is what bounds it: each lane keeps its own running maximum and sums (a new maximum
+// scales s and moves w: w' = a (w + s (m - m'))), and each wave the K best of what it has read.  A token is ordered by
+// one 64-bit key, the value's bits made monotonic above the complement of its index, so equal values fall to the
+// lower index, -0 equals 0 and NaN comes first.  A wave reads 1024 logits at a time; only keys above the K-th best so
+// far are looked at (until K are there: above the K-th best of the 64 lanes' best), collected in LDS and ranked by
+// counting.  A row goes to as many workgroups as fill the chip; a second kernel then joins their results.
+#include "v7g_device.h"
+#include "v7g_internal.h"
+
+namespace v7g {
+
+namespace {
+
+constexpr int kChunk = 1024;  // logits of one step of a wave, 16 a lane
+constexpr int kBest = 64;     // at most so many alternatives
+typedef unsigned long long Key;
+typedef float f4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// Never 0, which stands for no token.
+__device__ __forceinline__ Key make_key(float x, unsigned index) {
+  uint32_t b = __builtin_bit_cast(uint32_t, x);
+  if (b == 0x80000000u) b = 0;
+  b = (b & 0x7fffffffu) > 0x7f800000u ? 0xffffffffu : ((b & 0x80000000u) ? ~b : b | 0x80000000u);
+  return ((Key)b << 32) | (0xffffffffu - index);
+}
+__device__ __forceinline__ float key_value(Key k) {
+  const uint32_t b = (uint32_t)(k >> 32);
+  return __builtin_bit_cast(float, b == 0xffffffffu ? 0x7fc00000u : ((b & 0x80000000u) ? b & 0x7fffffffu : ~b));
+}
+__device__ __forceinline__ int key_index(Key k) { return (int)(0xffffffffu - (uint32_t)k); }
+
+__device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+// The K-th largest of the lanes' keys: the largest key that K lanes reach, bit by bit.
+__device__ __forceinline__ Key kth_of_lanes(Key mine, int K) {
+  Key t = 0;
+  for (int b = 63; b >= 0; --b) {
+    const Key c = t | (1ull << b);
+    if (__popcll(__ballot(mine >= c)) >= K) t = c;
+  }
+  return t;
+}
+
+// A wave's K best keys, sorted, at the front of its LDS buffer [kBest + kChunk + kBest]; the room behind takes the
+// candidates of one step and the new list.
+struct Best {
+  Key *buf;
+  int K, n = 0;
+  Key worst = 0;  // the K-th key once there are K
+
+  // Keys of one step, N a lane.
+  template <int N>
+  __device__ __forceinline__ void add(const Key (&k)[N]) {
+    Key top = k[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = k[i] > top ? k[i] : top;
+    if (!__ballot(top > worst)) return;
+    Key bar = worst + 1;
+    if (n < K) {
+      const Key t = kth_of_lanes(top, K);
+      bar = t > 1 ? t : 1;
+    }
+    int cnt = n;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const unsigned long long hit = __ballot(k[i] >= bar);
+      if (hit) {
+        if (k[i] >= bar) buf[cnt + __builtin_amdgcn_mbcnt_hi((unsigned)(hit >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)hit, 0))] = k[i];
+        cnt += __popcll(hit);
+      }
+    }
+    rank(cnt);
+  }
+
+  // The K best of the buffer's first cnt keys become the list.
+  __device__ __forceinline__ void rank(int cnt) {
+    Key *fresh = buf + kBest + kChunk;
+    wave_lds_fence();
+    for (int i0 = 0; i0 < cnt; i0 += 64) {
+      const int i = i0 + __lane_id();
+      const Key mine = i < cnt ? buf[i] : 0;
+      int r = 0;
+      for (int j = 0; j < cnt; ++j) r += buf[j] > mine;
+      if (i < cnt && r < K) fresh[r] = mine;
+    }
+    wave_lds_fence();
+    n = cnt < K ? cnt : K;
+    if ((int)__lane_id() < n) buf[__lane_id()] = fresh[__lane_id()];
+    wave_lds_fence();
+    if (n == K) worst = buf[K - 1];
+  }
+};
+
+struct Sums {
+  float m = -__builtin_inff(), s = 0.0f, w = 0.0f;
+  // Moves the sums to another maximum nm >= m.
+  __device__ __forceinline__ void move(float nm) {
+    if (nm > m) {
+      if (m > -__builtin_inff()) {
+        const float d = m - nm, a = __expf(d);
+        w = a > 0.0f ? a * (w + s * d) : 0.0f;
+        s *= a;
+      }
+      m = nm;
+    }
+  }
+  __device__ __forceinline__ void join(float m2, float s2, float w2) {
+    Sums o;
+    o.m = m2, o.s = s2, o.w = w2;
+    const float nm = fmaxf(m, m2);
+    move(nm);
+    o.move(nm);
+    s += o.s;
+    w += o.w;
+  }
+  __device__ __forceinline__ void join_lanes() {
+    for (int x = 32; x; x >>= 1) {
+      const float m2 = xor_f(m, x), s2 = xor_f(s, x), w2 = xor_f(w, x);
+      join(m2, s2, w2);
+    }
+  }
+};
+
+struct LogprobArgs {
+  float *logprob, *entropy, *top_logprob;
+  int32_t *top_ids;
+  const float *logits;
+  long long stride;
+  const int32_t *ids;
+  int vocab, K, parts, steps;  // steps: 4-wave steps of a part
+  float *part_sums;            // [row, part, 4]
+  Key *part_keys;              // [row, part, K]
+};
+
+__device__ __forceinline__ void write_row(const LogprobArgs &a, long long row, const Sums &t, const Key *best) {
+  const float lse = logf(t.s);
+  const int lane = __lane_id();
+  if (lane == 0) {
+    const int id = a.ids[row];
+    float lp = __builtin_nanf("");  // no such token
+    if (id >= 0 && id < a.vocab) lp = (a.logits[row * a.stride + id] - t.m) - lse;
+    a.logprob[row] = lp;
+    a.entropy[row] = lse - t.w / t.s;
+  }
+  if (lane < a.K) {
+    a.top_logprob[row * a.K + lane] = (key_value(best[lane]) - t.m) - lse;
+    a.top_ids[row * a.K + lane] = key_index(best[lane]);
+  }
+}
+
+template <bool TOP>
+__global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
+  __shared__ Key keys[TOP ? 4 : 1][TOP ? kBest + kChunk + kBest : 1];
+  __shared__ float sums[4][3];
+  __shared__ int counts[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long long row = blockIdx.x / a.parts;
+  const int part = blockIdx.x % a.parts;
+  const float *x = a.logits + row * a.stride;
+  Sums t;
+  Best best{keys[TOP ? wave : 0], a.K};
+  long long at = ((long long)part * a.steps * 4 + wave) * kChunk + lane * 4;
+  auto load = [&](long long p, float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long q = p + i * 256;
+      if (q + 4 <= a.vocab) {
+        const f4_a4 y = __builtin_nontemporal_load(reinterpret_cast<const f4_a4 *>(x + q));
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[4 * i + c] = y[c];
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[4 * i + c] = q + c < a.vocab ? x[q + c] : -__builtin_inff();
+      }
+    }
+  };
+  float v[16], nv[16];
+  load(at, v);
+  for (int st = 0; st < a.steps; ++st, at += 4 * kChunk) {
+    if (at - lane * 4 >= a.vocab) break;
+    if (st + 1 < a.steps) load(at + 4 * kChunk, nv);
+    float mx = v[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, v[i]);
+    t.move(fmaxf(t.m, mx));
+    const float ref = t.m == -__builtin_inff() ? 0.0f : t.m;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float z = v[i] - ref, e = __expf(z);  // NaN and +Inf make s NaN, and with it every result of the row
+      t.s += e;
+      t.w += e > 0.0f ? e * z : 0.0f;
+    }
+    if constexpr (TOP) {
+      Key k[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const long long q = at + (i >> 2) * 256 + (i & 3);
+        k[i] = q < a.vocab ? make_key(v[i], (unsigned)q) : 0;
+      }
+      best.add(k);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = nv[i];
+  }
+  t.join_lanes();
+  if (lane == 0) {
+    sums[wave][0] = t.m, sums[wave][1] = t.s, sums[wave][2] = t.w;
+    counts[wave] = best.n;
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  for (int w = 1; w < 4; ++w) t.join(sums[w][0], sums[w][1], sums[w][2]);
+  if constexpr (TOP) {
+    int cnt = best.n;
+    for (int w = 1; w < 4; ++w) {
+      const int n = counts[w];
+      if (lane < n) best.buf[cnt + lane] = keys[w][lane];
+      cnt += n;
+    }
+    best.rank(cnt);
+  }
+  if (a.parts == 1) {
+    write_row(a, row, t, best.buf);
+    return;
+  }
+  const long long slot = row * a.parts + part;
+  if (lane == 0) {
+    float *p = a.part_sums + slot * 4;
+    p[0] = t.m, p[1] = t.s, p[2] = t.w;
+  }
+  if (TOP && lane < a.K) a.part_keys[slot * a.K + lane] = lane < best.n ? best.buf[lane] : 0;
+}
+
+template <bool TOP>
+__global__ __launch_bounds__(64) void logprobs_join_kernel(LogprobArgs a) {
+  __shared__ Key keys[TOP ? kBest + kChunk + kBest : 1];
+  const int lane = threadIdx.x;
+  const long long row = blockIdx.x;
+  Sums t;
+  for (int p = lane; p < a.parts; p += 64) {
+    const float *q = a.part_sums + (row * a.parts + p) * 4;
+    t.join(q[0], q[1], q[2]);
+  }
+  t.join_lanes();
+  Best best{keys, a.K};
+  if constexpr (TOP) {
+    const Key *in = a.part_keys + row * a.parts * a.K;
+    const int n = a.parts * a.K;
+    for (int i0 = 0; i0 < n; i0 += 64 * 8) {
+      Key k[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) k[i] = i0 + i * 64 + lane < n ? in[i0 + i * 64 + lane] : 0;
+      best.add(k);
+    }
+  }
+  write_row(a, row, t, best.buf);
+}
+
+}  // namespace
+
+// Parts of a row: as many as give 2048 workgroups, no smaller than one step of four waves.
+int logprobs_parts(int rows, int vocab) {
+  const long long steps = ((long long)vocab + 4 * kChunk - 1) / (4 * kChunk);
+  const long long parts = rows > 0 ? (2048 + rows - 1) / rows : 1;
+  return (int)(parts < steps ? parts : steps);
+}
+
+long long logprobs_workspace(int rows, int vocab, int top_k) {
+  const int parts = logprobs_parts(rows, vocab);
+  return parts == 1 ? 0 : (long long)rows * parts * (16 + 8LL * top_k);
+}
+
+void launch_token_logprobs(float *logprob, float *entropy, float *top_logprob, int32_t *top_ids, const float *logits,
+                           long long stride, const int32_t *ids, int rows, int vocab, int top_k, void *workspace,
+                           hipStream_t stream) {
+  LogprobArgs a{logprob, entropy, top_logprob, top_ids, logits, stride, ids, vocab, top_k};
+  const long long steps = ((long long)vocab + 4 * kChunk - 1) / (4 * kChunk);
+  a.parts = logprobs_parts(rows, vocab);
+  a.steps = (int)((steps + a.parts - 1) / a.parts);
+  a.parts = (int)((steps + a.steps - 1) / a.steps);
+  a.part_sums = static_cast<float *>(workspace);
+  a.part_keys = reinterpret_cast<Key *>(a.part_sums + (long long)rows * a.parts * 4);
+  const dim3 grid((unsigned)((long long)rows * a.parts));
+  if (top_k)
+    enqueue(logprobs_kernel<true>, grid, dim3(256), 0, stream, a);
+  else
+    enqueue(logprobs_kernel<false>, grid, dim3(256), 0, stream, a);
+  if (a.parts == 1) return;
+  if (top_k)
+    enqueue(logprobs_join_kernel<true>, dim3((unsigned)rows), dim3(64), 0, stream, a);
+  else
+    enqueue(logprobs_join_kernel<false>, dim3((unsigned)rows), dim3(64), 0, stream, a);
+}
+
+}  // namespace v7g

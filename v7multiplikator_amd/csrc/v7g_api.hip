@@ -985,11 +985,11 @@ int launch_attn(v7g::AttnArgs &a, const AttnPlan &p, int head_dim, bool paged, v
 }
 
 int check_pages(const v7g_kv_pages &g) {
-  if (g.n_layers <= 0 || g.n_pages < 0 || g.page_size < 16 || g.page_size > 65536 ||
+  if (g.n_layers <= 0 || g.n_layers > 16384 || g.n_pages < 0 || g.page_size < 16 || g.page_size > 65536 ||
       (g.page_size & (g.page_size - 1)) || g.n_kv_heads <= 0 || g.head_dim <= 0)
     return V7G_ERR_SHAPE;
   const long long row = (long long)g.n_kv_heads * g.head_dim;
-  if (row % 4 || row >= (1LL << 30) || bad_stride(g.token_stride, g.page_size, row)) return V7G_ERR_SHAPE;
+  if (row % 4 || row >= (1LL << 24) || bad_stride(g.token_stride, g.page_size, row)) return V7G_ERR_SHAPE;
   const long long page = (g.page_size - 1) * g.token_stride + row;
   if (g.page_stride % 4 || (g.n_pages > 1 && g.page_stride < page)) return V7G_ERR_SHAPE;
   const long long layer = (g.n_pages > 1 ? (g.n_pages - 1) * g.page_stride : 0) + page;
@@ -1106,6 +1106,134 @@ int v7g_attention_tree(float *out, long long out_stride, const float *q, long lo
   a.n_kv_heads = g.n_kv_heads, a.group = n_q_heads / g.n_kv_heads;
   a.scale_log2 = scale * 1.4426950408889634f;
   return launch_attn(a, p, g.head_dim, true, workspace);
+}
+
+// ---------------------------------------------------------------- pages
+
+// Block tables are indexed in 32 bits, and a sequence's positions too.
+static bool bad_table(const v7g_kv_pages &g, int n_seqs, int table_width) {
+  return n_seqs < 0 || table_width < 0 || (long long)table_width * g.page_size >= (1LL << 31) - 64 ||
+         (long long)n_seqs * table_width >= (1LL << 31);
+}
+
+int v7g_kv_pack_f16_pages(const v7g_kv_pages *pages, const float *k_src, const float *v_src, long long src_stride,
+                          const int32_t *block_table, int table_width, int n_seqs, const int32_t *positions,
+                          const int32_t *seqs, int n_tokens) {
+  if (!pages) return fail(V7G_ERR_NULL);
+  const v7g_kv_pages &g = *pages;
+  if (int rc = check_pages(g)) return fail(rc);
+  const long long row = (long long)g.n_kv_heads * g.head_dim;
+  if (n_tokens < 0 || bad_table(g, n_seqs, table_width) || bad_stride(src_stride, n_tokens, row))
+    return fail(V7G_ERR_SHAPE);
+  if (!seqs && n_tokens > n_seqs) return fail(V7G_ERR_SHAPE);
+  if (n_tokens == 0 || n_seqs == 0 || table_width == 0 || g.n_pages == 0) return V7G_OK;
+  if (!k_src || !v_src || !block_table || !positions) return fail(V7G_ERR_NULL);
+  if (!al16(k_src) || !al16(v_src) || (((uintptr_t)block_table | (uintptr_t)positions | (uintptr_t)seqs) & 3u))
+    return fail(V7G_ERR_ALIGN);
+  if (int ac = check_alias({pages_span(g, g.k, 1), pages_span(g, g.v, 1)},
+                           {v7g::row_span(k_src, n_tokens, src_stride * 4, row * 4),
+                            v7g::row_span(v_src, n_tokens, src_stride * 4, row * 4),
+                            v7g::flat_span(block_table, 4LL * n_seqs * table_width),
+                            v7g::flat_span(positions, 4LL * n_tokens), v7g::flat_span(seqs, 4LL * n_tokens)}))
+    return fail(ac);
+  if (int pc = check_ptrs({g.k, g.v, k_src, v_src, block_table, positions, seqs})) return fail(pc);
+  v7g::launch_kv_pack_pages(g, k_src, v_src, src_stride, block_table, table_width, n_seqs, positions, seqs, n_tokens,
+                            stream());
+  return check_launch();
+}
+
+int64_t v7g_kv_pages_assign_workspace(int n_seqs, int n_pages) {
+  return n_seqs < 0 || n_pages < 0 ? 0 : v7g::kv_assign_workspace(n_seqs, n_pages);
+}
+
+int v7g_kv_pages_assign(const v7g_kv_pages *pages, int32_t *table_out, int32_t *lens_out, int32_t *refs_out,
+                        int32_t *short_out, const int32_t *block_table, const int32_t *lens, const int32_t *refs,
+                        const int32_t *parents, const int32_t *reserve, int n_seqs, int table_width, void *workspace,
+                        int64_t workspace_bytes) {
+  if (!pages) return fail(V7G_ERR_NULL);
+  const v7g_kv_pages &g = *pages;
+  if (int rc = check_pages(g)) return fail(rc);
+  if (bad_table(g, n_seqs, table_width)) return fail(V7G_ERR_SHAPE);
+  const long long need = v7g::kv_assign_workspace(n_seqs, g.n_pages), entries = (long long)n_seqs * table_width;
+  if (!short_out || (g.n_pages && (!refs || !refs_out)) || (n_seqs && (!lens_out || !lens || !parents)) ||
+      (entries && (!table_out || !block_table)) || (need && !workspace))
+    return fail(V7G_ERR_NULL);
+  if (workspace_bytes < need) return fail(V7G_ERR_SHAPE);
+  if ((((uintptr_t)table_out | (uintptr_t)lens_out | (uintptr_t)refs_out | (uintptr_t)short_out |
+        (uintptr_t)block_table | (uintptr_t)lens | (uintptr_t)refs | (uintptr_t)parents | (uintptr_t)reserve) & 3u) ||
+      !al16(workspace))
+    return fail(V7G_ERR_ALIGN);
+  const long long rb = 4LL * n_seqs, pb = 4LL * g.n_pages;
+  if (int ac = check_alias({pages_span(g, g.k, g.n_layers), pages_span(g, g.v, g.n_layers),
+                            v7g::flat_span(table_out, 4 * entries), v7g::flat_span(lens_out, rb),
+                            v7g::flat_span(refs_out, pb), v7g::flat_span(short_out, 4),
+                            v7g::flat_span(workspace, need)},
+                           {v7g::flat_span(block_table, 4 * entries), v7g::flat_span(lens, rb),
+                            v7g::flat_span(refs, pb), v7g::flat_span(parents, rb), v7g::flat_span(reserve, rb)}))
+    return fail(ac);
+  if (int pc = check_ptrs({g.k, g.v, table_out, lens_out, refs_out, short_out, block_table, lens, refs, parents,
+                           reserve, workspace}))
+    return fail(pc);
+  v7g::launch_kv_assign(g, table_out, lens_out, refs_out, short_out, block_table, lens, refs, parents, reserve, n_seqs,
+                        table_width, workspace, stream());
+  return check_launch();
+}
+
+int v7g_kv_pages_compact(const v7g_kv_pages *pages, int32_t *lens_out, const int32_t *block_table, int table_width,
+                         const int32_t *lens, const int32_t *path, int path_width, const int32_t *n_path, int n_seqs) {
+  if (!pages) return fail(V7G_ERR_NULL);
+  const v7g_kv_pages &g = *pages;
+  if (int rc = check_pages(g)) return fail(rc);
+  if (bad_table(g, n_seqs, table_width) || path_width < 0 || (long long)n_seqs * path_width >= (1LL << 31))
+    return fail(V7G_ERR_SHAPE);
+  if (n_seqs == 0) return V7G_OK;
+  if (!lens_out || !lens || !n_path || (path_width && !path) || (table_width && !block_table))
+    return fail(V7G_ERR_NULL);
+  if (((uintptr_t)lens_out | (uintptr_t)block_table | (uintptr_t)lens | (uintptr_t)path | (uintptr_t)n_path) & 3u)
+    return fail(V7G_ERR_ALIGN);
+  const long long rb = 4LL * n_seqs;
+  if (int ac = check_alias({pages_span(g, g.k, g.n_layers), pages_span(g, g.v, g.n_layers),
+                            v7g::flat_span(lens_out, rb)},
+                           {v7g::flat_span(block_table, rb * table_width), v7g::flat_span(lens, rb),
+                            v7g::flat_span(path, rb * path_width), v7g::flat_span(n_path, rb)}))
+    return fail(ac);
+  if (int pc = check_ptrs({g.k, g.v, lens_out, block_table, lens, path, n_path})) return fail(pc);
+  v7g::launch_kv_compact(g, block_table, table_width, n_seqs, lens, path, path_width, n_path, lens_out, stream());
+  return check_launch();
+}
+
+// ---------------------------------------------------------------- token scores
+
+int64_t v7g_token_logprobs_workspace(int n_tokens, int vocab, int top_k) {
+  return n_tokens < 0 || vocab <= 0 || top_k < 0 ? 0 : v7g::logprobs_workspace(n_tokens, vocab, top_k);
+}
+
+int v7g_token_logprobs(float *logprob, float *entropy, float *top_logprob, int32_t *top_ids, const float *logits,
+                       long long stride, const int32_t *ids, int n_tokens, int vocab, int top_k, void *workspace,
+                       int64_t workspace_bytes) {
+  if (n_tokens < 0 || vocab <= 0 || vocab > (1 << 30) || top_k < 0 || top_k > 64 || top_k > vocab)
+    return fail(V7G_ERR_SHAPE);
+  if (n_tokens > 1 && stride < vocab) return fail(V7G_ERR_SHAPE);
+  if (n_tokens == 0) return V7G_OK;
+  const long long need = v7g::logprobs_workspace(n_tokens, vocab, top_k);
+  if (!logprob || !entropy || !logits || !ids || (top_k && (!top_logprob || !top_ids)) || (need && !workspace))
+    return fail(V7G_ERR_NULL);
+  if (workspace_bytes < need) return fail(V7G_ERR_SHAPE);
+  if ((((uintptr_t)logprob | (uintptr_t)entropy | (uintptr_t)logits | (uintptr_t)ids) & 3u) || !al16(workspace) ||
+      (top_k && (((uintptr_t)top_logprob | (uintptr_t)top_ids) & 3u)))
+    return fail(V7G_ERR_ALIGN);
+  const long long tb = 4LL * n_tokens;
+  if (int ac = check_alias({v7g::flat_span(logprob, tb), v7g::flat_span(entropy, tb),
+                            v7g::flat_span(top_logprob, tb * top_k), v7g::flat_span(top_ids, tb * top_k),
+                            v7g::flat_span(need ? workspace : nullptr, need)},
+                           {v7g::row_span(logits, n_tokens, stride * 4, 4LL * vocab), v7g::flat_span(ids, tb)}))
+    return fail(ac);
+  if (int pc = check_ptrs({logprob, entropy, top_k ? top_logprob : nullptr, top_k ? top_ids : nullptr, logits, ids,
+                           need ? workspace : nullptr}))
+    return fail(pc);
+  v7g::launch_token_logprobs(logprob, entropy, top_logprob, top_ids, logits, stride, ids, n_tokens, vocab, top_k,
+                             workspace, stream());
+  return check_launch();
 }
 
 }  // extern "C"

@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "../../include/v7g_lib.h"
+
 namespace v7g {
 
 // Timing events armed by v7g_time_next_call for the calling host thread.  The
@@ -89,5 +91,24 @@ int arith_selfcheck(unsigned long long mismatches[4], hipStream_t stream);
 // mismatches[w] for the selected identities only.  Synchronous; returns 0 or
 // -1 on a HIP error.
 int arith_selfcheck_noalloc(unsigned long long mismatches[4], int checks, hipStream_t stream);
+
+// token_logprobs: workspace in bytes, and the launch.
+long long logprobs_workspace(int rows, int vocab, int top_k);
+void launch_token_logprobs(float *logprob, float *entropy, float *top_logprob, int32_t *top_ids, const float *logits,
+                           long long stride, const int32_t *ids, int rows, int vocab, int top_k, void *workspace,
+                           hipStream_t stream);
+
+// The pages of a K/V cache.
+void launch_kv_pack_pages(const v7g_kv_pages &g, const float *k_src, const float *v_src, long long src_stride,
+                          const int32_t *table, int width, int n_seqs, const int32_t *positions, const int32_t *seqs,
+                          int tokens, hipStream_t stream);
+void launch_kv_compact(const v7g_kv_pages &g, const int32_t *table, int width, int rows, const int32_t *lens,
+                       const int32_t *path, int path_width, const int32_t *n_path, int32_t *lens_out,
+                       hipStream_t stream);
+long long kv_assign_workspace(int rows, int n_pages);
+void launch_kv_assign(const v7g_kv_pages &g, int32_t *table_out, int32_t *lens_out, int32_t *refs_out,
+                      int32_t *short_out, const int32_t *table, const int32_t *lens, const int32_t *refs,
+                      const int32_t *parents, const int32_t *reserve, int rows, int width, void *workspace,
+                      hipStream_t stream);
 
 }  // namespace v7g

@@ -2,7 +2,7 @@
 
 Mirrors the reference's kernel entry points (src/v7_lib.h:113-128,269-281) for
 batched device tensors.  Every function validates its tensors, binds the
-library to torch's current stream and makes ONE launch through the C ABI of
+library to torch's current stream and makes ONE call through the C ABI of
 libv7g.so; nothing runs on the CPU and there is no fallback: without the built
 library the first call raises.
 
@@ -23,6 +23,9 @@ library the first call raises.
   kv_pack_f16_kv     <- v7s_kv_pack_f16 for K then V (src/asm/forward_q8.inc:345-358), one launch
   rope_only_heads    <- v7s_rope_only_heads     (src/asm/rope_only_dispatch.inc:11-47)
   qkv_rope_stage     <- the per-token Q/K/V stage of the prefill, one launch (src/asm/prefill_q8.inc:848-883)
+
+Around the K/V cache, with no reference export of these forms (a call makes one launch, or a few where pieces are
+joined): attention_prefill, attention_tree, kv_pack_f16_pages, kv_pages_assign, kv_pages_compact, token_logprobs.
 """
 from __future__ import annotations
 
@@ -699,3 +702,106 @@ def attention_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                               words if T else 0, B, T, Hq, _scale(scale, D), _ptr(ws), 0 if ws is None else ws.numel())
     _lib.check(rc, "attention_tree")
     return out
+
+
+def kv_pack_f16_pages(k_src: torch.Tensor, v_src: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                      block_table: torch.Tensor, positions: torch.Tensor, seqs: torch.Tensor | None = None) -> None:
+    """binary16 copies of the K and V rows [T, Hk*D] f32 (views into one fused QKV buffer: the same row stride) into
+    one layer's pages [n_pages, page_size, Hk, D]: token t's at position positions[t] of the sequence of block table
+    row seqs[t] (None: row t).  A token with no such row, position or page is skipped; the places of one call are
+    distinct."""
+    _need(k_src, torch.float32, "k_src", contiguous=False)
+    _need(v_src, torch.float32, "v_src", contiguous=False)
+    if k_src.dim() != 2 or k_src.stride(1) != 1 or v_src.shape != k_src.shape or v_src.stride() != k_src.stride():
+        raise ValueError("k_src and v_src must be [tokens, row_len] with contiguous rows and the same row stride")
+    g = _kv_pages(k_pages, v_pages, False)
+    T, n = k_src.shape
+    if n != g.n_kv_heads * g.head_dim:
+        raise ValueError("a row must hold the pages' kv_heads*head_dim floats")
+    _table(block_table, None)
+    _rows_i32(positions, T, "positions")
+    B, W = block_table.shape
+    if seqs is not None:
+        _rows_i32(seqs, T, "seqs")
+    elif T > B:
+        raise ValueError("without seqs there is at most one token per sequence")
+    _bind(k_src)
+    rc = _lib.load().v7g_kv_pack_f16_pages(ctypes.addressof(g), k_src.data_ptr(), v_src.data_ptr(), k_src.stride(0),
+                                           block_table.data_ptr(), W, B, positions.data_ptr(), _ptr(seqs), T)
+    _lib.check(rc, "kv_pack_f16_pages")
+
+
+def kv_pages_assign(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
+                    refs: torch.Tensor, parents: torch.Tensor, reserve: torch.Tensor | None = None):
+    """Forks, frees and grows the sequences of a paged cache: returns (block_table, lens, refs, short), all new.
+
+    Row r of the new table [B, W] is the sequence of row parents[r] (r: stays, another row: a fork, -1: freed), with
+    room for reserve[r] more tokens.  Full pages are shared and counted in refs [n_pages] (0: free); a partly filled
+    last page is copied, in every layer of k_pages, v_pages [(layers,) n_pages, page_size, Hk, D], for every row but
+    the one that takes it over (the parent itself, else its lowest fork).  New pages are the lowest free ones, in the
+    order of the rows; short [1] counts those that were missing, whose entries stay -1 (a fork without its copy ends
+    with its full pages).  All indices int32."""
+    g = _kv_pages(k_pages, v_pages, True)
+    _table(block_table, None)
+    B, W = block_table.shape
+    _rows_i32(lens, B, "lens")
+    _rows_i32(refs, g.n_pages, "refs")
+    _rows_i32(parents, B, "parents")
+    if reserve is not None:
+        _rows_i32(reserve, B, "reserve")
+    table_out, lens_out, refs_out = torch.empty_like(block_table), torch.empty_like(lens), torch.empty_like(refs)
+    short = torch.empty(1, dtype=torch.int32, device=refs.device)
+    L = _lib.load()
+    ws = _workspace(L.v7g_kv_pages_assign_workspace(B, g.n_pages), refs.device)
+    _bind(refs)
+    rc = L.v7g_kv_pages_assign(ctypes.addressof(g), table_out.data_ptr(), lens_out.data_ptr(), refs_out.data_ptr(),
+                               short.data_ptr(), block_table.data_ptr(), lens.data_ptr(), refs.data_ptr(),
+                               parents.data_ptr(), _ptr(reserve), B, W, _ptr(ws), 0 if ws is None else ws.numel())
+    _lib.check(rc, "kv_pages_assign")
+    return table_out, lens_out, refs_out, short
+
+
+def kv_pages_compact(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
+                     path: torch.Tensor, n_path: torch.Tensor) -> torch.Tensor:
+    """Keeps accepted drafts: of the new tokens behind lens[r] tokens of row r, those numbered path[r, :n_path[r]]
+    (strictly ascending; the path ends at the first entry that does not ascend or has no page) move to the places from
+    lens[r] on, in every layer of k_pages, v_pages [(layers,) n_pages, page_size, Hk, D].  Returns the new lens."""
+    g = _kv_pages(k_pages, v_pages, True)
+    _table(block_table, None)
+    B, W = block_table.shape
+    _rows_i32(lens, B, "lens")
+    _rows_i32(n_path, B, "n_path")
+    _table(path, B, "path")
+    lens_out = torch.empty_like(lens)
+    _bind(lens)
+    rc = _lib.load().v7g_kv_pages_compact(ctypes.addressof(g), lens_out.data_ptr(), block_table.data_ptr(), W,
+                                          lens.data_ptr(), path.data_ptr(), path.shape[1], n_path.data_ptr(), B)
+    _lib.check(rc, "kv_pages_compact")
+    return lens_out
+
+
+def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0):
+    """Scores of logit rows [T, V] f32 (row stride free): returns (logprobs [T] of the tokens ids [T] int32, entropies
+    [T] in nats, top log probabilities [T, top_k], top ids [T, top_k] int32; top_k <= 64).  Equal logits: the lower
+    index first.  An id outside the vocabulary gives NaN, a row with NaN or +inf or nothing above -inf NaN for every
+    probability."""
+    _need(logits, torch.float32, "logits", contiguous=False)
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be [tokens, vocab] with contiguous rows")
+    T, V = logits.shape
+    _rows_i32(ids, T, "ids")
+    K = int(top_k)
+    if not 0 <= K <= 64:
+        raise ValueError("top_k must lie in 0..64")
+    dev = logits.device
+    lp, ent = (torch.empty(T, dtype=torch.float32, device=dev) for _ in range(2))
+    tl = torch.empty((T, K), dtype=torch.float32, device=dev)
+    ti = torch.empty((T, K), dtype=torch.int32, device=dev)
+    L = _lib.load()
+    ws = _workspace(L.v7g_token_logprobs_workspace(T, V, K), dev)
+    _bind(logits)
+    rc = L.v7g_token_logprobs(lp.data_ptr(), ent.data_ptr(), tl.data_ptr() if K else None, ti.data_ptr() if K else None,
+                              logits.data_ptr(), logits.stride(0), ids.data_ptr(), T, V, K, _ptr(ws),
+                              0 if ws is None else ws.numel())
+    _lib.check(rc, "token_logprobs")
+    return lp, ent, tl, ti
