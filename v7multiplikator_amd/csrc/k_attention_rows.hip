@@ -46,10 +46,6 @@ __device__ __forceinline__ void load_slice(const uint16_t *p, uint32_t (&v)[4]) 
   }
 }
 
-__device__ __forceinline__ bool nonfinite16(uint32_t x) {
-  return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u;
-}
-
 // A operand of tile t of a slice: the pairs of keys at element t.
 __device__ __forceinline__ v4u v_tile(const uint32_t (&v)[8][4], int t) {
   const unsigned sel = (t & 1) ? 0x07060302u : 0x05040100u;
@@ -281,59 +277,47 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
     load_k(b);
     v4f sc[2];
     scores(sc);
-    // which of this lane's keys a row sees, given the row's limit and token
-    auto seen_by = [&](int lim_n, const int64_t *words_n) {
-      unsigned bits = 0;
+    // which of this lane's keys its row sees
+    unsigned seen = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3), d = key - s.off;
-        bool on = key < lim_n;
-        if (tree && !on) on = d < a.mask_words * 64 && ((words_n[d >> 6] >> (d & 63)) & 1);
-        if (on && key < key_hi && b.ok[j >> 2]) bits |= 1u << j;
-      }
-      return bits;
-    };
-    const unsigned seen = seen_by(lim, words);
+    for (int j = 0; j < 8; ++j) {
+      const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3), d = key - s.off;
+      bool on = key < lim;
+      if (tree && !on) on = d < a.mask_words * 64 && ((words[d >> 6] >> (d & 63)) & 1);
+      if (on && key < key_hi && b.ok[j >> 2]) seen |= 1u << j;
+    }
     float x[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = (seen >> j) & 1 ? sc[j >> 2][j & 3] * factor : -__builtin_inff();
     weigh(x);
-    // 0 * Inf would carry an infinite or NaN element of a V row to rows that do not see its key: keys that no row
-    // may read stand for zeros, and where others hold such elements the rows are taken one at a time.
+    // keys that no row may read stand for zeros, whatever their V rows hold
     each(slices, [&](auto i) {
       constexpr int W = S::width(i);
       uint32_t v[8][4];
       load_v(b, i, v);
-      bool bad = false;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int d = 0; d < W / 2; ++d) {
+        for (int d = 0; d < W / 2; ++d)
           if (kb + 16 * (j >> 2) + 4 * g + (j & 3) >= key_hi || !b.ok[j >> 2]) v[j][d] = 0;
-          bad |= nonfinite16(v[j][d]);
-        }
-      if (!__ballot(bad)) {
-        add_slice(i, v);
-        return;
-      }
-      for (int n = 0; n < 16; ++n) {
-        const int tok_n = __shfl(tok, n);
-        const unsigned seen_n = seen_by(__shfl(lim, n), a.mask + (long long)(s.q0 + tok_n) * a.mask_words);
 #pragma unroll
-        for (int t = 0; t < W; ++t) {
-          v4u f = v_tile(v, t);
-#pragma unroll
-          for (int jj = 0; jj < 4; ++jj)
-            f[jj] &= ((seen_n >> (2 * jj)) & 1 ? 0xffffu : 0u) | ((seen_n >> (2 * jj + 1)) & 1 ? 0xffff0000u : 0u);
-          const v8h v8 = __builtin_bit_cast(v8h, f);
+      for (int t = 0; t < W; ++t) {
+        v4f &o = acc[S::tile(i) + t];
+        v8h v8 = __builtin_bit_cast(v8h, v_tile(v, t));
+        if (__ballot(any_nonfinite(v8))) {
+          const v8h sees = seen_part(seen);
           const v4f z = {0, 0, 0, 0};
-          const v4f r = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph, acc[S::tile(i) + t], 0, 0, 0);
-          // a zero lo part times an infinite element is no result: hi's product decides there
-          const v4f r2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl, z, 0, 0, 0);
+          const v4f up = __builtin_amdgcn_mfma_f32_16x16x32_f16(infinite_part(v8, false), sees, z, 0, 0, 0);
+          const v4f down = __builtin_amdgcn_mfma_f32_16x16x32_f16(infinite_part(v8, true), sees, z, 0, 0, 0);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (c == n) acc[S::tile(i) + t][k] = __builtin_fabsf(r2[k]) < __builtin_inff() ? r[k] + r2[k] : r[k];
+          for (int k = 0; k < 4; ++k) {
+            o[k] += up[k] > 0.0f ? __builtin_inff() : 0.0f;
+            o[k] -= down[k] > 0.0f ? __builtin_inff() : 0.0f;
+          }
+          v8 = finite_part(v8);
         }
+        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph, o, 0, 0, 0);
+        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl, o, 0, 0, 0);
       }
     });
   }
@@ -436,32 +420,36 @@ void rows_launch(const AttnArgs &a, bool paged, unsigned grid, hipStream_t strea
 
 }  // namespace
 
-void launch_attention(const AttnArgs &a, int head_dim, bool paged, long long units, bool split, hipStream_t stream) {
+void launch_attention(const AttnArgs &a, int head_dim, bool paged, int tile_rows, long long units, bool split,
+                      hipStream_t stream) {
   const unsigned grid = (unsigned)(units * a.n_kv_heads);
-  switch (head_dim) {
-    case 64: rows_launch<64>(a, paged, grid, stream); break;
-    case 96: rows_launch<96>(a, paged, grid, stream); break;
-    case 128: rows_launch<128>(a, paged, grid, stream); break;
-    case 160: rows_launch<160>(a, paged, grid, stream); break;
-    case 192: rows_launch<192>(a, paged, grid, stream); break;
-    case 224: rows_launch<224>(a, paged, grid, stream); break;
-    case 256: rows_launch<256>(a, paged, grid, stream); break;
-    case 288: rows_launch<288>(a, paged, grid, stream); break;
-    case 320: rows_launch<320>(a, paged, grid, stream); break;
-    case 352: rows_launch<352>(a, paged, grid, stream); break;
-    case 384: rows_launch<384>(a, paged, grid, stream); break;
-    case 416: rows_launch<416>(a, paged, grid, stream); break;
-    case 448: rows_launch<448>(a, paged, grid, stream); break;
-    case 480: rows_launch<480>(a, paged, grid, stream); break;
-    case 512: rows_launch<512>(a, paged, grid, stream); break;
-  }
+  if (tile_rows == kAttnTileRows)
+    launch_attention_tiles(a, head_dim, paged, grid, stream);
+  else
+    switch (head_dim) {
+      case 64: rows_launch<64>(a, paged, grid, stream); break;
+      case 96: rows_launch<96>(a, paged, grid, stream); break;
+      case 128: rows_launch<128>(a, paged, grid, stream); break;
+      case 160: rows_launch<160>(a, paged, grid, stream); break;
+      case 192: rows_launch<192>(a, paged, grid, stream); break;
+      case 224: rows_launch<224>(a, paged, grid, stream); break;
+      case 256: rows_launch<256>(a, paged, grid, stream); break;
+      case 288: rows_launch<288>(a, paged, grid, stream); break;
+      case 320: rows_launch<320>(a, paged, grid, stream); break;
+      case 352: rows_launch<352>(a, paged, grid, stream); break;
+      case 384: rows_launch<384>(a, paged, grid, stream); break;
+      case 416: rows_launch<416>(a, paged, grid, stream); break;
+      case 448: rows_launch<448>(a, paged, grid, stream); break;
+      case 480: rows_launch<480>(a, paged, grid, stream); break;
+      case 512: rows_launch<512>(a, paged, grid, stream); break;
+    }
   if (split) {
     const long long waves = (long long)a.n_tokens * a.n_kv_heads * a.group;
     const unsigned blocks = (unsigned)((waves + 3) / 4);
     if (paged)
-      enqueue(attention_join_kernel<true>, dim3(blocks), dim3(256), 0, stream, a, head_dim, 16);
+      enqueue(attention_join_kernel<true>, dim3(blocks), dim3(256), 0, stream, a, head_dim, tile_rows);
     else
-      enqueue(attention_join_kernel<false>, dim3(blocks), dim3(256), 0, stream, a, head_dim, 16);
+      enqueue(attention_join_kernel<false>, dim3(blocks), dim3(256), 0, stream, a, head_dim, tile_rows);
   }
 }
 

@@ -33,7 +33,9 @@ struct AttnArgs {
   float *part_ml;    // [unit, KV head, tile row, 2]: running maximum (log2 domain) and sum
 };
 
-constexpr int kAttnRowTile = 16;    // rows of a tile
+constexpr int kAttnRowTile = 16;    // rows of a tile of the few-row kernel
+constexpr int kAttnTileRows = 128;  // rows of a tile of the many-row kernel
+constexpr int kAttnTileDims = 256;  // the many-row kernel's widest head
 constexpr int kAttnUnits = 1024;    // units that fill the chip: four workgroups for each of 256 compute units
 constexpr int kAttnMinChunk = 256;  // keys; shorter pieces cost more in joining than they save
 
@@ -134,13 +136,16 @@ __device__ __forceinline__ bool attn_find(const AttnArgs &a, int tile_rows, int 
       u.s.off = __builtin_amdgcn_readlane(s.off, l);
       u.pieces = __builtin_amdgcn_readlane(pieces, l);
       const int first = base + __builtin_amdgcn_readlane(incl - units, l);
+      const int tiles = (int)(((long long)u.s.nq * a.group + tile_rows - 1) / tile_rows);
+      // a sequence's last tiles see the most keys: they come first
       if (of_token >= 0) {
         u.tile = (int)(((long long)(of_token - u.s.q0) * a.group + row_in_token) / tile_rows);
         u.piece = 0;
-        want = first + u.tile * u.pieces;
+        want = first + (tiles - 1 - u.tile) * u.pieces;
       } else {
-        u.tile = (want - first) / u.pieces;
-        u.piece = (want - first) - u.tile * u.pieces;
+        const int t = (want - first) / u.pieces;
+        u.tile = tiles - 1 - t;
+        u.piece = (want - first) - t * u.pieces;
       }
       return true;
     }
@@ -177,12 +182,53 @@ __device__ __forceinline__ void split8(const float (&x)[8], v8h &hi, v8h &lo) {
   }
 }
 
+// Infinities and NaN among the binary16 elements of a V operand.  Rows that do not see such an element's key must not
+// meet it as 0 * Inf, so where a mask cuts, these elements go as zeros into the product with the weights, and a second
+// pair of products counts, per row and element, the +Inf and -Inf (NaN: both) among the keys that the row does see.
+__device__ __forceinline__ bool nonfinite16(uint32_t x) {
+  return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u;
+}
+__device__ __forceinline__ bool any_nonfinite(v8h v) {
+  const v4u w = __builtin_bit_cast(v4u, v);
+  return nonfinite16(w[0]) || nonfinite16(w[1]) || nonfinite16(w[2]) || nonfinite16(w[3]);
+}
+__device__ __forceinline__ v8h finite_part(v8h v) {
+  v8h r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint16_t b = __builtin_bit_cast(uint16_t, (_Float16)v[i]);
+    r[i] = (b & 0x7c00u) == 0x7c00u ? (_Float16)0.0f : (_Float16)v[i];
+  }
+  return r;
+}
+// 1 for an infinity of the sign and for NaN, else 0.
+__device__ __forceinline__ v8h infinite_part(v8h v, bool negative) {
+  v8h r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint16_t b = __builtin_bit_cast(uint16_t, (_Float16)v[i]);
+    const bool on = b == (negative ? 0xfc00u : 0x7c00u) || (b & 0x7fffu) > 0x7c00u;
+    r[i] = (_Float16)(on ? 1.0f : 0.0f);
+  }
+  return r;
+}
+// 1 for each of the lane's 8 keys whose bit is set.
+__device__ __forceinline__ v8h seen_part(unsigned bits) {
+  v8h r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = (_Float16)((bits >> i) & 1 ? 1.0f : 0.0f);
+  return r;
+}
+
 // Softmax weights are 2^(score - reference + 4): the reference follows the running maximum only when a score
 // passes it by more than 8, so weights reach 2^12 at most and lo keeps its bits for weights near 1.
 constexpr float kAttnWeightShift = 4.0f;
 constexpr float kAttnLazy = 8.0f;
 
-// Shapes and pointers are validated by the caller; units: at most, per KV head; split: pieces have to be joined.
-void launch_attention(const AttnArgs &a, int head_dim, bool paged, long long units, bool split, hipStream_t stream);
+// Shapes and pointers are validated by the caller; tile_rows is kAttnRowTile or kAttnTileRows, units at most the units
+// per KV head, split: pieces have to be joined.
+void launch_attention(const AttnArgs &a, int head_dim, bool paged, int tile_rows, long long units, bool split,
+                      hipStream_t stream);
+void launch_attention_tiles(const AttnArgs &a, int head_dim, bool paged, unsigned grid, hipStream_t stream);
 
 }  // namespace v7g
