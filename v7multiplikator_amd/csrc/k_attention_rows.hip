@@ -12,8 +12,6 @@
 //     the first tile (j < 4) or 4g+j-4 of the second.  Lane (g, c) loads a slice of its 8 keys' V rows (16 bytes at
 //     head_dim 128: 16 lanes read 256 bytes of a row); the row index c of tile t then stands for element 8c+t, and
 //     the A operand of every tile comes from the lane's own registers with one v_perm per pair of keys.
-#include <utility>
-
 #include "v7g_attention.h"
 #include "v7g_internal.h"
 
@@ -55,11 +53,6 @@ __device__ __forceinline__ v4u v_tile(const uint32_t (&v)[8][4], int t) {
   return f;
 }
 
-template <int... I, class F>
-__device__ __forceinline__ void each(std::integer_sequence<int, I...>, F f) {
-  (f(std::integral_constant<int, I>{}), ...);
-}
-
 template <int D, bool PAGED>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(AttnArgs a) {
   using S = VSlices<D>;
@@ -73,7 +66,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
   const int hk = blockIdx.x % a.n_kv_heads;
   int unit = blockIdx.x / a.n_kv_heads;
   AttnUnit u;
-  if (!attn_find<PAGED>(a, 16, unit, -1, 0, u)) return;
+  if (!attn_find<PAGED>(a, kAttnRowShift, unit, -1, 0, u)) return;
   const AttnSeq s = u.s;
   const int rows = s.nq * a.group, row0 = u.tile * 16;
   const int n_rows = rows - row0 < 16 ? rows - row0 : 16;
@@ -374,38 +367,68 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
   });
 }
 
-// Joins the pieces of the rows whose keys were cut: one wave per (token, query head).
+// Joins the pieces of the rows whose keys were cut: one wave per (token, query head).  The pieces' weights come from
+// one read of all their maxima, a lane each (64 at a time); the accumulators are then read 8 pieces at a time.
 template <bool PAGED>
-__global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, int head_dim, int tile_rows) {
+__global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, int head_dim, int shift) {
   const int lane = threadIdx.x & 63;
-  const int heads = a.n_kv_heads * a.group;
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= (long long)a.n_tokens * heads) return;
-  const int tok = (int)(w / heads), head = (int)(w % heads);
-  const int hk = head / a.group, hr = head % a.group;
+  const unsigned heads = a.n_kv_heads * a.group;
+  const unsigned w = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (w >= (unsigned)a.n_tokens * heads) return;
+  const int tok = (int)(w / heads), head = (int)(w - (w / heads) * heads);
+  const int hk = head / a.group, hr = head - hk * a.group;
   int unit = 0;
   AttnUnit u;
-  if (!attn_find<PAGED>(a, tile_rows, unit, tok, hr, u) || u.pieces == 1) return;
-  const int r = (int)(((long long)(tok - u.s.q0) * a.group + hr) % tile_rows);
-  auto slot = [&](int p) { return (((long long)unit + p) * a.n_kv_heads + hk) * tile_rows + r; };
-  float m = -__builtin_inff();
-  for (int p = lane; p < u.pieces; p += 64) m = fmaxf(m, a.part_ml[slot(p) * 2]);
-  for (int x = 32; x; x >>= 1) m = fmaxf(m, xor_f(m, x));
-  const float ref = m == -__builtin_inff() ? 0.0f : m;
-  float l = 0.0f;
-  float o[8] = {0, 0, 0, 0, 0, 0, 0, 0};  // head_dim <= 512
-  for (int p = 0; p < u.pieces; ++p) {
-    const long long sl = slot(p);
-    const float wgt = __builtin_amdgcn_exp2f(a.part_ml[sl * 2] - ref);  // an empty piece: 2^-inf = 0
-    l += wgt * a.part_ml[sl * 2 + 1];
+  if (!attn_find<PAGED>(a, shift, unit, tok, hr, u) || u.pieces == 1) return;
+  const int r = ((tok - u.s.q0) * a.group + hr) & ((1 << shift) - 1);
+  // slot of piece p: the tile's row r in unit + p
+  const long long slot0 = ((((long long)unit * a.n_kv_heads + hk) << shift) + r);
+  const long long step = (long long)a.n_kv_heads << shift;
+  float m = -__builtin_inff(), l = 0.0f;
+  constexpr int NV = 8;  // head_dim <= 512
+  float o[NV] = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int p0 = 0; p0 < u.pieces; p0 += 64) {
+    float mp = -__builtin_inff(), lp = 0.0f;
+    if (p0 + lane < u.pieces) {
+      const float *ml = a.part_ml + (slot0 + (p0 + lane) * step) * 2;
+      mp = ml[0], lp = ml[1];
+    }
+    float top = mp;
+    for (int x = 32; x; x >>= 1) top = fmaxf(top, xor_f(top, x));
+    const float nm = fmaxf(m, top);
+    if (nm > -__builtin_inff()) {
+      const float alpha = __builtin_amdgcn_exp2f(m - nm);
+      l *= alpha;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 64 * i < head_dim) o[i] += wgt * a.part_o[sl * head_dim + lane + 64 * i];
+      for (int i = 0; i < NV; ++i) o[i] *= alpha;
+      m = nm;
+    }
+    const float ref = m == -__builtin_inff() ? 0.0f : m;
+    const float wgt = __builtin_amdgcn_exp2f(mp - ref);  // an empty piece: 2^-inf = 0
+    float sum = wgt * lp;
+    for (int x = 32; x; x >>= 1) sum += xor_f(sum, x);
+    l += sum;
+    const int n = u.pieces - p0 < 64 ? u.pieces - p0 : 64;
+    for (int p = 0; p < n; p += 8) {
+      float v[8][NV];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float *src = a.part_o + (slot0 + (p0 + (p + j < n ? p + j : n - 1)) * step) * head_dim;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[j][i] = lane + 64 * i < head_dim ? src[lane + 64 * i] : 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float wj = p + j < n ? __shfl(wgt, p + j) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) o[i] += wj * v[j][i];
+      }
+    }
   }
   const float mul = l == 0.0f ? 0.0f : 1.0f / l;
   float *dst = a.out + (long long)tok * a.out_stride + (long long)head * head_dim;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < NV; ++i)
     if (lane + 64 * i < head_dim) dst[lane + 64 * i] = o[i] * mul;
 }
 
@@ -420,10 +443,10 @@ void rows_launch(const AttnArgs &a, bool paged, unsigned grid, hipStream_t strea
 
 }  // namespace
 
-void launch_attention(const AttnArgs &a, int head_dim, bool paged, int tile_rows, long long units, bool split,
+void launch_attention(const AttnArgs &a, int head_dim, bool paged, int shift, long long units, bool split,
                       hipStream_t stream) {
   const unsigned grid = (unsigned)(units * a.n_kv_heads);
-  if (tile_rows == kAttnTileRows)
+  if (shift == kAttnTileShift)
     launch_attention_tiles(a, head_dim, paged, grid, stream);
   else
     switch (head_dim) {
@@ -447,9 +470,9 @@ void launch_attention(const AttnArgs &a, int head_dim, bool paged, int tile_rows
     const long long waves = (long long)a.n_tokens * a.n_kv_heads * a.group;
     const unsigned blocks = (unsigned)((waves + 3) / 4);
     if (paged)
-      enqueue(attention_join_kernel<true>, dim3(blocks), dim3(256), 0, stream, a, head_dim, tile_rows);
+      enqueue(attention_join_kernel<true>, dim3(blocks), dim3(256), 0, stream, a, head_dim, shift);
     else
-      enqueue(attention_join_kernel<false>, dim3(blocks), dim3(256), 0, stream, a, head_dim, tile_rows);
+      enqueue(attention_join_kernel<false>, dim3(blocks), dim3(256), 0, stream, a, head_dim, shift);
   }
 }
 

@@ -13,8 +13,6 @@
 //     two transposing LDS reads of 4 keys each.
 // LDS rows are padded by 16 bytes (K) and 32 bytes (V): the 8 K rows that one pass of 16-byte reads touches, and the 4
 // V rows of one transposing read, then start on different banks.
-#include <utility>
-
 #include "v7g_attention.h"
 #include "v7g_internal.h"
 
@@ -28,7 +26,9 @@ template <int D>
 struct TileLds {
   static constexpr int krow = D + 8, vrow = D + 16;  // elements
   static constexpr int side = kKeys * (krow + vrow);
-  static constexpr int bytes = 2 * side * 2;
+  // The widest heads leave no registers for the lower part of q: it waits in LDS, each wave's own.
+  static constexpr bool q_low = D >= 224;
+  static constexpr int bytes = 2 * side * 2 + (q_low ? kAttnTileRows * D * 2 : 0);
 };
 
 // Elements d0..d0+15 of 4 keys, transposed: lane i of 16 gets element d0+i of the 4 keys; it hands in the address of
@@ -51,13 +51,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
   using L = TileLds<D>;
   constexpr int KS = D / 16, DT = D / 32, CR = D / 8;
   constexpr int NL = (kKeys * CR + 255) / 256;  // 16-byte pieces of a K tile per thread
+  constexpr auto pieces = std::make_integer_sequence<int, NL>{};
   extern __shared__ _Float16 tile_lds[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int h = lane >> 5, c = lane & 31;
   const int hk = blockIdx.x % a.n_kv_heads;
   int unit = blockIdx.x / a.n_kv_heads;
   AttnUnit u;
-  if (!attn_find<PAGED>(a, kAttnTileRows, unit, -1, 0, u)) return;
+  if (!attn_find<PAGED>(a, kAttnTileShift, unit, -1, 0, u)) return;
   const AttnSeq s = u.s;
   const int row0 = u.tile * kAttnTileRows + wave * 32;
   const int left = s.nq * a.group - row0;
@@ -78,7 +79,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
   const int key_hi = u.piece + 1 < u.pieces ? min((u.piece + 1) * u.piece_keys, tile_max) : tile_max;
 
   // ---- q rows in two binary16 parts; the scale's sign goes with them, so that the largest product is the maximum
-  v8h qh[KS], ql[KS];
+  v8h qh[KS], ql[L::q_low ? 1 : KS];
+  v8h *qlow = reinterpret_cast<v8h *>(tile_lds + 2 * L::side) + wave * KS * 64 + lane;
   float factor;
   {
     const float *qr = a.q + (long long)(s.q0 + tok) * a.q_stride + (long long)head * D + h * 8;
@@ -97,7 +99,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
       float x[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = __builtin_ldexpf(qr[ks * 16 + i], e) * sign;
-      split8(x, qh[ks], ql[ks]);
+      v8h low;
+      split8(x, qh[ks], low);
+      if constexpr (L::q_low)
+        qlow[ks * 64] = low;
+      else
+        ql[ks] = low;
     }
   }
 
@@ -121,41 +128,63 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
     }
   };
   v4u kreg[NL], vreg[NL];
-  // K and V rows of keys kb.. into registers; keys of no row or no page become zeros
-  auto fetch = [&](int kb, const int (&pg)[2]) {
+  // where a thread's pieces of the step to fetch next lie: packed rows are walked from step to step, paged ones
+  // within 16 keys of a page
+  long long ko[NL], vo[NL];
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int idx = threadIdx.x + i * 256;
-      const int r = idx / CR, ch = idx % CR, key = kb + r;
-      kreg[i] = vreg[i] = v4u{0, 0, 0, 0};
-      bool on = key < key_hi && (NL * 256 == kKeys * CR || r < kKeys);
-      long long ko, vo;
-      if constexpr (PAGED) {
-        const int p = r < 16 ? pg[0] : pg[1];
-        on = on && p >= 0;
-        const int in = key & ((1 << a.page_shift) - 1);
-        ko = p * a.page_stride + in * a.k_stride;
-        vo = p * a.page_stride + in * a.v_stride;
-      } else {
-        ko = (long long)(s.kv0 + key) * a.k_stride;
-        vo = (long long)(s.kv0 + key) * a.v_stride;
+  for (int i = 0; i < NL; ++i) {
+    const int idx = threadIdx.x + i * 256, r = idx / CR, ch = idx % CR;
+    const long long first = PAGED ? (r & 15) : s.kv0 + key_lo + r;
+    ko[i] = first * a.k_stride + ch * 8;
+    vo[i] = first * a.v_stride + ch * 8;
+  }
+  const long long kstep = kKeys * a.k_stride, vstep = kKeys * a.v_stride;
+  // K and V rows of keys kb.. into registers; keys of no row or no page become zeros (read at the step's first row,
+  // or in page 0)
+  auto fetch = [&](int kb, const int (&pg)[2]) {
+    const uint16_t *k0 = kbase, *k1 = kbase, *v0 = vbase, *v1 = vbase;
+    if constexpr (PAGED) {
+      const int in0 = kb & ((1 << a.page_shift) - 1), in1 = (kb + 16) & ((1 << a.page_shift) - 1);
+      const long long p0 = max(pg[0], 0) * a.page_stride, p1 = max(pg[1], 0) * a.page_stride;
+      k0 += p0 + in0 * a.k_stride;
+      v0 += p0 + in0 * a.v_stride;
+      k1 += p1 + in1 * a.k_stride;
+      v1 += p1 + in1 * a.v_stride;
+    }
+    const bool whole = kb + kKeys <= key_hi && (!PAGED || (pg[0] >= 0 && pg[1] >= 0));
+    each(pieces, [&](auto i) {
+      const int idx = threadIdx.x + i * 256, r = idx / CR, ch = idx % CR;
+      const bool inside = kb + r < key_hi && (NL * 256 == kKeys * CR || r < kKeys);
+      const uint16_t *kp = (PAGED && r >= 16 ? k1 : k0) + ko[i], *vp = (PAGED && r >= 16 ? v1 : v0) + vo[i];
+      if (!inside) {
+        kp = (PAGED ? k0 : k0 + ko[i] - r * a.k_stride) + (PAGED ? ch * 8 : 0);
+        vp = (PAGED ? v0 : v0 + vo[i] - r * a.v_stride) + (PAGED ? ch * 8 : 0);
       }
-      if (on) {
-        kreg[i] = *reinterpret_cast<const v4u_a8 *>(kbase + ko + ch * 8);
-        vreg[i] = *reinterpret_cast<const v4u_a8 *>(vbase + vo + ch * 8);
+      kreg[i] = *reinterpret_cast<const v4u_a8 *>(kp);
+      vreg[i] = *reinterpret_cast<const v4u_a8 *>(vp);
+      if constexpr (!PAGED) {
+        ko[i] += kstep;
+        vo[i] += vstep;
       }
+    });
+    if (!whole) {
+      each(pieces, [&](auto i) {
+        const int r = (threadIdx.x + i * 256) / CR;
+        const bool on = kb + r < key_hi && (!PAGED || (r < 16 ? pg[0] : pg[1]) >= 0);
+        kreg[i] = on ? kreg[i] : v4u{0, 0, 0, 0};
+        vreg[i] = on ? vreg[i] : v4u{0, 0, 0, 0};
+      });
     }
   };
   auto store = [&](_Float16 *buf) {
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
+    each(pieces, [&](auto i) {
       const int idx = threadIdx.x + i * 256;
       const int r = idx / CR, ch = idx % CR;
       if (NL * 256 == kKeys * CR || r < kKeys) {
         *reinterpret_cast<v4u *>(buf + r * L::krow + ch * 8) = kreg[i];
         *reinterpret_cast<v4u *>(buf + kKeys * L::krow + r * L::vrow + ch * 8) = vreg[i];
       }
-    }
+    });
   };
 
   // One step on a buffer; bit i of gone: its keys 16i.. are on no page.  CUT: the mask, the piece's end or the last key
@@ -170,7 +199,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
     for (int ks = 0; ks < KS; ++ks) {
       const v8h k8 = *reinterpret_cast<const v8h *>(kl + ks * 16);
       sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, qh[ks], sc, 0, 0, 0);
-      sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, ql[ks], sc, 0, 0, 0);
+      sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, L::q_low ? qlow[ks * 64] : ql[L::q_low ? 0 : ks], sc, 0, 0, 0);
     }
     unsigned seen = 0xffffu;  // of this lane's 16 keys, those its row sees
     if constexpr (CUT) {

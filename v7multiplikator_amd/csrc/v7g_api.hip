@@ -946,7 +946,7 @@ namespace {
 // How a call is cut: tiles of rows, and pieces of their keys where the tiles alone leave compute units idle.
 // max_keys is the most keys a sequence can have, as far as the host knows.
 struct AttnPlan {
-  int tile_rows = 0;
+  int shift = 0;  // tiles of 2^shift rows
   int target = 0;         // units per KV head aimed at, 0: whole tiles
   long long units = 0;    // at most, per KV head
   long long workspace = 0;
@@ -955,13 +955,13 @@ struct AttnPlan {
 AttnPlan attn_plan(int n_seqs, int n_tokens, int group, int n_kv_heads, int head_dim, long long max_keys) {
   AttnPlan p;
   const long long rows = (long long)n_tokens * group;
-  p.tile_rows = head_dim <= v7g::kAttnTileDims && rows > 32LL * n_seqs ? v7g::kAttnTileRows : v7g::kAttnRowTile;
-  const long long tiles = rows / p.tile_rows + n_seqs;
+  p.shift = head_dim <= v7g::kAttnTileDims && rows > 32LL * n_seqs ? v7g::kAttnTileShift : v7g::kAttnRowShift;
+  const long long tiles = (rows >> p.shift) + n_seqs;
   p.units = tiles;
   if (tiles * n_kv_heads < v7g::kAttnUnits && max_keys > v7g::kAttnMinChunk) {
     p.target = (v7g::kAttnUnits + n_kv_heads - 1) / n_kv_heads;
     p.units = tiles + p.target;
-    p.workspace = p.units * n_kv_heads * p.tile_rows * (head_dim + 2) * 4;
+    p.workspace = ((p.units * n_kv_heads) << p.shift) * (head_dim + 2) * 4;
   }
   return p;
 }
@@ -971,7 +971,7 @@ int check_attention(int n_seqs, int n_tokens, int n_q_heads, int n_kv_heads, int
     return V7G_ERR_SHAPE;
   if (head_dim < 64 || head_dim > 512 || head_dim % 32 != 0) return V7G_ERR_SHAPE;
   if ((long long)n_tokens * n_q_heads >= (1LL << 31) - 64 || n_seqs >= (1 << 30)) return V7G_ERR_SHAPE;
-  const long long tiles = (long long)n_tokens * (n_q_heads / n_kv_heads) / v7g::kAttnRowTile + n_seqs;
+  const long long tiles = ((long long)n_tokens * (n_q_heads / n_kv_heads) >> v7g::kAttnRowShift) + n_seqs;
   return (tiles + v7g::kAttnUnits) * n_kv_heads >= (1LL << 31) ? V7G_ERR_SHAPE : V7G_OK;
 }
 
@@ -982,8 +982,8 @@ bool bad_stride(long long stride, long long rows, long long row_len) {
 int launch_attn(v7g::AttnArgs &a, const AttnPlan &p, int head_dim, bool paged, void *workspace) {
   a.split_target = p.target;
   a.part_o = static_cast<float *>(workspace);
-  a.part_ml = a.part_o ? a.part_o + p.units * a.n_kv_heads * p.tile_rows * head_dim : nullptr;
-  v7g::launch_attention(a, head_dim, paged, p.tile_rows, p.units, p.target != 0, stream());
+  a.part_ml = a.part_o ? a.part_o + ((p.units * a.n_kv_heads) << p.shift) * head_dim : nullptr;
+  v7g::launch_attention(a, head_dim, paged, p.shift, p.units, p.target != 0, stream());
   return check_launch();
 }
 

@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <utility>
+
 #include "v7g_device.h"
 
 namespace v7g {
@@ -33,8 +35,9 @@ struct AttnArgs {
   float *part_ml;    // [unit, KV head, tile row, 2]: running maximum (log2 domain) and sum
 };
 
-constexpr int kAttnRowTile = 16;    // rows of a tile of the few-row kernel
-constexpr int kAttnTileRows = 128;  // rows of a tile of the many-row kernel
+constexpr int kAttnRowShift = 4;    // 16 rows make a tile of the few-row kernel
+constexpr int kAttnTileShift = 7;   // 128 rows one of the many-row kernel
+constexpr int kAttnTileRows = 1 << kAttnTileShift;
 constexpr int kAttnTileDims = 256;  // the many-row kernel's widest head
 constexpr int kAttnUnits = 1024;    // units that fill the chip: four workgroups for each of 256 compute units
 constexpr int kAttnMinChunk = 256;  // keys; shorter pieces cost more in joining than they save
@@ -77,57 +80,63 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs &a, int b) {
   return s;
 }
 
-// A unit of work: TM rows of a sequence and one piece of its keys.
+// A unit of work: a tile of rows of a sequence and one piece of its keys.
 struct AttnUnit {
   AttnSeq s;
   int seq, tile, piece, pieces, piece_keys;
 };
 
-__device__ __forceinline__ int lane_id() { return __lane_id(); }
+// Sum over the wave's lanes, in every lane.
+__device__ __forceinline__ int wave_sum(int v) {
+  v += (int)dpp_u<DPP_QUAD_XOR1>((uint32_t)v);
+  v += (int)dpp_u<DPP_QUAD_XOR2>((uint32_t)v);
+  v += (int)dpp_u<DPP_ROW_HALF_MIRROR>((uint32_t)v);
+  v += (int)dpp_u<DPP_ROW_MIRROR>((uint32_t)v);
+  const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+  v = (int)(a[0] + a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+  return (int)(b[0] + b[1]);
+}
+
+// Tiles of 2^shift rows that a sequence has (tokens times heads stay below 2^31, the entry's check).
+__device__ __forceinline__ int attn_tiles(const AttnSeq &s, int group, int shift) {
+  return (int)(((unsigned)(s.nq * group) + (1u << shift) - 1) >> shift);
+}
 
 // Keys per piece: the summed key counts of all tiles over the units aimed at, in whole blocks of 64.  Every
 // workgroup derives the same number from the lengths, so the host needs none of them.
 template <bool PAGED>
-__device__ __forceinline__ int attn_piece_keys(const AttnArgs &a, int tile_rows) {
-  if (!a.split_target) return 0x7fffffff;
+__device__ __forceinline__ int attn_piece_keys(const AttnArgs &a, int shift) {
   long long sum = 0;
-  for (int b = lane_id(); b < a.n_seqs; b += 64) {
+  for (int b = __lane_id(); b < a.n_seqs; b += 64) {
     const AttnSeq s = attn_seq<PAGED>(a, b);
-    sum += (long long)(((long long)s.nq * a.group + tile_rows - 1) / tile_rows) * s.kv;
+    sum += (long long)attn_tiles(s, a.group, shift) * s.kv;
   }
   for (int m = 32; m; m >>= 1) sum += __shfl_xor(sum, m);
-  long long keys = (sum + a.split_target - 1) / a.split_target;
-  keys = (keys + 63) & ~63ll;
-  return keys < kAttnMinChunk ? kAttnMinChunk : (keys > 0x7fffffc0 ? 0x7fffffff : (int)keys);
+  const long long keys = sum / a.split_target + 1;
+  return keys < kAttnMinChunk ? kAttnMinChunk : (keys > 0x7fffff00 ? 0x7fffffff : ((int)keys + 63) & ~63);
 }
 
-// Unit number `want` in the order of sequences, tiles and pieces; with `of_token` the unit of that token's row
-// instead (its first piece), its number returned in `want`.  False: past the last.  Every lane of the wave takes part.
+// Unit number `want`; with of_token >= 0 instead the unit of row row_in_token of that token (its first piece), whose
+// number is returned in `want`.  False: past the last.  Every lane of the wave takes part.  Units go by sequences,
+// tiles from the last (which sees the most keys) to the first, and pieces; where nothing is cut and one step of the
+// wave's lanes holds all sequences, by tiles first, the longest of all sequences to the shortest.
 template <bool PAGED>
-__device__ __forceinline__ bool attn_find(const AttnArgs &a, int tile_rows, int &want, int of_token, int row_in_token,
+__device__ __forceinline__ bool attn_find(const AttnArgs &a, int shift, int &want, int of_token, int row_in_token,
                                           AttnUnit &u) {
-  u.piece_keys = attn_piece_keys<PAGED>(a, tile_rows);
+  u.piece_keys = a.split_target ? attn_piece_keys<PAGED>(a, shift) : 0x7fffffff;
+  const int lane = __lane_id();
   int base = 0;
   for (int b0 = 0; b0 < a.n_seqs; b0 += 64) {
-    const int b = b0 + lane_id();
+    const int b = b0 + lane;
     AttnSeq s{0, 0, 0, 0, 0};
-    int units = 0, pieces = 1;
+    int tiles = 0, pieces = 1;
     if (b < a.n_seqs) {
       s = attn_seq<PAGED>(a, b);
-      const int tiles = (int)(((long long)s.nq * a.group + tile_rows - 1) / tile_rows);
-      pieces = s.kv <= u.piece_keys ? 1 : (int)(((long long)s.kv + u.piece_keys - 1) / u.piece_keys);
-      units = tiles * pieces;
+      tiles = attn_tiles(s, a.group, shift);
+      pieces = s.kv <= u.piece_keys ? 1 : (int)(((unsigned)s.kv + (unsigned)u.piece_keys - 1) / (unsigned)u.piece_keys);
     }
-    int incl = units;
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(incl, d);
-      if (lane_id() >= d) incl += o;
-    }
-    const bool mine = of_token >= 0 ? (of_token >= s.q0 && of_token < s.q0 + s.nq)
-                                    : (want >= base + incl - units && want < base + incl);
-    const unsigned long long hit = __ballot(mine);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
+    auto take = [&](int l) {
       u.seq = b0 + l;
       u.s.q0 = __builtin_amdgcn_readlane(s.q0, l);
       u.s.nq = __builtin_amdgcn_readlane(s.nq, l);
@@ -135,16 +144,49 @@ __device__ __forceinline__ bool attn_find(const AttnArgs &a, int tile_rows, int 
       u.s.kv = __builtin_amdgcn_readlane(s.kv, l);
       u.s.off = __builtin_amdgcn_readlane(s.off, l);
       u.pieces = __builtin_amdgcn_readlane(pieces, l);
+    };
+    if (!a.split_target && a.n_seqs > 1 && a.n_seqs <= 64) {
+      // from(t): the units of tiles t and later, which come before all others
+      auto from = [&](int t) { return wave_sum(tiles > t ? tiles - t : 0); };
+      if (want >= from(0)) return false;
+      int lo = 0, hi = 1;
+      while (from(hi) > want) lo = hi, hi *= 2;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (from(mid) > want)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      const unsigned long long has = __ballot(tiles > lo);
+      const int nth = want - from(lo + 1);
+      const bool mine = tiles > lo && __popcll(has & ((1ull << lane) - 1)) == nth;
+      take(__builtin_ctzll(__ballot(mine)));
+      u.tile = lo;
+      u.piece = 0;
+      return true;
+    }
+    const int units = tiles * pieces;
+    int incl = units;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(incl, d);
+      if (lane >= d) incl += o;
+    }
+    const bool mine = of_token >= 0 ? (of_token >= s.q0 && of_token < s.q0 + s.nq)
+                                    : (want >= base + incl - units && want < base + incl);
+    const unsigned long long hit = __ballot(mine);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      take(l);
       const int first = base + __builtin_amdgcn_readlane(incl - units, l);
-      const int tiles = (int)(((long long)u.s.nq * a.group + tile_rows - 1) / tile_rows);
-      // a sequence's last tiles see the most keys: they come first
+      const int n = __builtin_amdgcn_readlane(tiles, l);
       if (of_token >= 0) {
-        u.tile = (int)(((long long)(of_token - u.s.q0) * a.group + row_in_token) / tile_rows);
+        u.tile = ((of_token - u.s.q0) * a.group + row_in_token) >> shift;
         u.piece = 0;
-        want = first + (tiles - 1 - u.tile) * u.pieces;
+        want = first + (n - 1 - u.tile) * u.pieces;
       } else {
-        const int t = (want - first) / u.pieces;
-        u.tile = tiles - 1 - t;
+        const int t = (int)((unsigned)(want - first) / (unsigned)u.pieces);
+        u.tile = n - 1 - t;
         u.piece = (want - first) - t * u.pieces;
       }
       return true;
@@ -152,6 +194,12 @@ __device__ __forceinline__ bool attn_find(const AttnArgs &a, int tile_rows, int 
     base += __builtin_amdgcn_readlane(incl, 63);
   }
   return false;
+}
+
+// f(0), f(1), ... with the indices as constants.
+template <int... I, class F>
+__device__ __forceinline__ void each(std::integer_sequence<int, I...>, F f) {
+  (f(std::integral_constant<int, I>{}), ...);
 }
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -175,10 +223,19 @@ __device__ __forceinline__ int q_row_exponent(float row_max) {
 }
 
 __device__ __forceinline__ void split8(const float (&x)[8], v8h &hi, v8h &lo) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    hi[i] = (_Float16)x[i];
-    lo[i] = (_Float16)(x[i] - (float)hi[i]);
+  for (int i = 0; i < 8; i += 2) {
+    const v2h h = __builtin_convertvector((v2f{x[i], x[i + 1]}), v2h);
+    // x - h, exact, as fused multiply-adds that take their binary16 operand without a conversion (from the source
+    // they become two instructions each)
+    v2f d;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d[0]) : "v"(h), "v"(x[i]));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d[1]) : "v"(h), "v"(x[i + 1]));
+    const v2h r = __builtin_convertvector(d, v2h);
+    hi[i] = h[0], hi[i + 1] = h[1];
+    lo[i] = r[0], lo[i + 1] = r[1];
   }
 }
 
@@ -225,9 +282,9 @@ __device__ __forceinline__ v8h seen_part(unsigned bits) {
 constexpr float kAttnWeightShift = 4.0f;
 constexpr float kAttnLazy = 8.0f;
 
-// Shapes and pointers are validated by the caller; tile_rows is kAttnRowTile or kAttnTileRows, units at most the units
-// per KV head, split: pieces have to be joined.
-void launch_attention(const AttnArgs &a, int head_dim, bool paged, int tile_rows, long long units, bool split,
+// Shapes and pointers are validated by the caller; tiles hold 2^shift rows (kAttnRowShift or kAttnTileShift), units: at
+// most, per KV head, split: pieces have to be joined.
+void launch_attention(const AttnArgs &a, int head_dim, bool paged, int shift, long long units, bool split,
                       hipStream_t stream);
 void launch_attention_tiles(const AttnArgs &a, int head_dim, bool paged, unsigned grid, hipStream_t stream);
 
