@@ -57,16 +57,18 @@ template <int D, bool PAGED>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(AttnArgs a) {
   using S = VSlices<D>;
   constexpr int KS = D / 32, NT = D / 16;
-  constexpr bool QREG = D <= 128;   // q in registers; wider heads read it from LDS, which all four waves share
-  constexpr bool AHEAD = D <= 256;  // the next block's K and V rows are loaded while this one is computed
+  // Two blocks' K and V rows fit in registers: one is computed while the other is on its way (8 waves of a compute
+  // unit keep 16 KB each in flight at head_dim 128).  Wider heads load each slice as it is used.
+  constexpr bool AHEAD = D <= 256;
   constexpr auto slices = std::make_integer_sequence<int, S::count>{};
   extern __shared__ float lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15;
-  const int hk = blockIdx.x % a.n_kv_heads;
-  int unit = blockIdx.x / a.n_kv_heads;
+  // heads first: workgroups that run at the same time read different pages (37 sequences: 182 -> 169 us against the
+  // other order, 64 of 1000-4000 keys 158 -> 148)
+  int hk, unit = blockIdx.x;
   AttnUnit u;
-  if (!attn_find<PAGED>(a, kAttnRowShift, unit, -1, 0, u)) return;
+  if (!attn_find<PAGED, FIND_HEADS_FIRST>(a, kAttnRowShift, unit, hk, u)) return;
   const AttnSeq s = u.s;
   const int rows = s.nq * a.group, row0 = u.tile * 16;
   const int n_rows = rows - row0 < 16 ? rows - row0 : 16;
@@ -83,8 +85,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
   const int key_hi = u.piece + 1 < u.pieces ? min((u.piece + 1) * u.piece_keys, lim_max) : lim_max;
   const int full_hi = min(key_hi, lim_min);  // up to here every row sees every key
 
-  // ---- q rows, scaled by a power of two and split in two binary16 parts
-  v8h qh[QREG ? KS : 1], ql[QREG ? KS : 1];
+  // ---- q rows, scaled by a power of two and split in two binary16 parts; in LDS, where all four waves read them
   v8h *qlds = reinterpret_cast<v8h *>(lds);  // [KS][2][64]
   float factor;
   {
@@ -99,20 +100,17 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
     const int e = q_row_exponent(mx);
     factor = __builtin_ldexpf(a.scale_log2, -e);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      float x[8];
+    for (int ks = 0; ks < KS; ++ks)
+      if (ks % 4 == wave) {
+        float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __builtin_ldexpf(qr[ks * 32 + i], e);
-      v8h hi, lo;
-      split8(x, hi, lo);
-      if constexpr (QREG) {
-        qh[ks] = hi, ql[ks] = lo;
-      } else if (wave == 0) {
+        for (int i = 0; i < 8; ++i) x[i] = __builtin_ldexpf(qr[ks * 32 + i], e);
+        v8h hi, lo;
+        split8(x, hi, lo);
         qlds[(ks * 2) * 64 + lane] = hi;
         qlds[(ks * 2 + 1) * 64 + lane] = lo;
       }
-    }
-    if constexpr (!QREG) __syncthreads();
+    __syncthreads();
   }
 
   v4f acc[NT];
@@ -135,8 +133,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
       const int key0 = h && b.last < 16 ? kb : kb + 16 * h;
       b.ok[h] = true;
       if constexpr (PAGED) {
-        int page = a.table[(long long)u.seq * a.table_width + (key0 >> a.page_shift)];
-        page = __builtin_amdgcn_readfirstlane(page);
+        int page = page_entry(a.table, (long long)u.seq * a.table_width + (key0 >> a.page_shift));
         b.ok[h] = (unsigned)page < (unsigned)a.n_pages;  // a page outside the pool: its keys are absent
         if (!b.ok[h]) page = 0;
         const int in = key0 & ((1 << a.page_shift) - 1);
@@ -149,35 +146,47 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
     }
     return b;
   };
-  auto half_last = [&](const Block &b, int h) { return h && b.last >= 16 ? b.last - 16 : min(b.last, 15); };
 
-  v4u kr[2][KS];
-  auto load_k = [&](const Block &b) {
+  // One block's rows in registers.
+  struct Rows {
+    v4u k[2][KS];
+    uint32_t v[AHEAD ? S::count : 1][8][4];
+    bool ok[2];
+  };
+  // Row offsets of a whole block (all 32 keys inside); CUT: rows behind the last key are read at that key.
+  const long long k_row = c * a.k_stride + g * 8, v_row = 4 * g * a.v_stride;
+  auto load_k = [&](auto cut, const Block &b, v4u (&k)[2][KS]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint16_t *r = b.k[h] + (long long)min(c, half_last(b, h)) * a.k_stride + g * 8;
+      const uint16_t *r = b.k[h] + k_row;
+      if constexpr (cut) {
+        const int last = h && b.last >= 16 ? b.last - 16 : min(b.last, 15);
+        r = b.k[h] + (long long)min(c, last) * a.k_stride + g * 8;
+      }
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) kr[h][ks] = *reinterpret_cast<const v4u_a8 *>(r + ks * 32);
+      for (int ks = 0; ks < KS; ++ks) k[h][ks] = *reinterpret_cast<const v4u_a8 *>(r + ks * 32);
     }
   };
-  uint32_t vr[AHEAD ? S::count : 1][8][4];
-  auto load_v = [&](const Block &b, auto i, uint32_t (&v)[8][4]) {
+  auto load_v = [&](auto cut, const Block &b, auto i, uint32_t (&v)[8][4]) {
     constexpr int W = S::width(i);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint16_t *r = b.v[j >> 2] + (long long)min(4 * g + (j & 3), half_last(b, j >> 2)) * a.v_stride;
+      const uint16_t *r = b.v[j >> 2] + v_row + (j & 3) * a.v_stride;
+      if constexpr (cut) {
+        const int last = j >= 4 && b.last >= 16 ? b.last - 16 : min(b.last, 15);
+        r = b.v[j >> 2] + (long long)min(4 * g + (j & 3), last) * a.v_stride;
+      }
       load_slice<W>(r + S::base(i) + c * W, v[j]);
     }
   };
-  auto scores = [&](v4f (&sc)[2]) {
+  auto scores = [&](const v4u (&k)[2][KS], v4f (&sc)[2]) {
     sc[0] = sc[1] = v4f{0, 0, 0, 0};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      const v8h hi = QREG ? qh[QREG ? ks : 0] : qlds[(ks * 2) * 64 + lane];
-      const v8h lo = QREG ? ql[QREG ? ks : 0] : qlds[(ks * 2 + 1) * 64 + lane];
+      const v8h hi = qlds[(ks * 2) * 64 + lane], lo = qlds[(ks * 2 + 1) * 64 + lane];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const v8h k8 = __builtin_bit_cast(v8h, kr[h][ks]);
+        const v8h k8 = __builtin_bit_cast(v8h, k[h][ks]);
         sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, hi, sc[h], 0, 0, 0);
         sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, lo, sc[h], 0, 0, 0);
       }
@@ -217,59 +226,68 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
   };
 
   // ---- blocks whose keys every row sees
-  int kb = key_lo + wave * 32;
-  if (kb + 32 <= full_hi) {
-    Block b = block_at(kb);
-    if constexpr (AHEAD) {
-      load_k(b);
-      each(slices, [&](auto i) { load_v(b, i, vr[i]); });
+  constexpr auto whole = std::false_type{};
+  constexpr auto cut = std::true_type{};
+  auto load = [&](int kb, Rows &r) {
+    const Block b = block_at(kb);
+    r.ok[0] = b.ok[0], r.ok[1] = b.ok[1];
+    load_k(whole, b, r.k);
+    if constexpr (AHEAD) each(slices, [&](auto i) { load_v(whole, b, i, r.v[i]); });
+  };
+  auto compute = [&](int kb, Rows &r) {
+    v4f sc[2];
+    scores(r.k, sc);
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = sc[j >> 2][j & 3] * factor;
+    const bool gone = PAGED && (!r.ok[0] || !r.ok[1]);
+    if (gone) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (!r.ok[j >> 2]) x[j] = -__builtin_inff();
     }
-    while (true) {
-      if constexpr (!AHEAD) load_k(b);
-      v4f sc[2];
-      scores(sc);
-      const bool more = kb + 128 + 32 <= full_hi;
-      Block nb = b;
-      if (more) {
-        nb = block_at(kb + 128);
-        if constexpr (AHEAD) load_k(nb);
+    weigh(x);
+    each(slices, [&](auto i) {
+      auto &v = r.v[AHEAD ? i : 0];
+      if constexpr (!AHEAD) load_v(whole, block_at(kb), i, v);
+      if (gone) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            if (!r.ok[j >> 2]) v[j][d] = 0;
       }
-      float x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = sc[j >> 2][j & 3] * factor;
-      if constexpr (PAGED)
-        if (!b.ok[0] || !b.ok[1]) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (!b.ok[j >> 2]) x[j] = -__builtin_inff();
-        }
-      weigh(x);
-      each(slices, [&](auto i) {
-        auto &v = vr[AHEAD ? i : 0];
-        if constexpr (!AHEAD) load_v(b, i, v);
-        if constexpr (PAGED)
-          if (!b.ok[0] || !b.ok[1]) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-              for (int d = 0; d < 4; ++d)
-                if (!b.ok[j >> 2]) v[j][d] = 0;
-          }
-        add_slice(i, v);
-        if constexpr (AHEAD)
-          if (more) load_v(nb, i, v);
-      });
+      add_slice(i, v);
+    });
+  };
+  int kb = key_lo + wave * 32;
+  if constexpr (AHEAD) {
+    Rows ra, rb;
+    if (kb + 32 <= full_hi) load(kb, ra);
+    while (kb + 32 <= full_hi) {
+      const bool second = kb + 160 <= full_hi;
+      if (second) load(kb + 128, rb);
+      compute(kb, ra);
       kb += 128;
-      if (!more) break;
-      b = nb;
+      if (!second) break;
+      if (kb + 160 <= full_hi) load(kb + 128, ra);
+      compute(kb, rb);
+      kb += 128;
+    }
+  } else {
+    for (; kb + 32 <= full_hi; kb += 128) {
+      Rows r;
+      load(kb, r);
+      compute(kb, r);
     }
   }
   // ---- blocks that the mask, the piece's end or the last key cuts
   for (; kb < key_hi; kb += 128) {
     const Block b = block_at(kb);
-    load_k(b);
+    v4u k[2][KS];
+    load_k(cut, b, k);
     v4f sc[2];
-    scores(sc);
+    scores(k, sc);
     // which of this lane's keys its row sees
     unsigned seen = 0;
 #pragma unroll
@@ -287,7 +305,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
     each(slices, [&](auto i) {
       constexpr int W = S::width(i);
       uint32_t v[8][4];
-      load_v(b, i, v);
+      load_v(cut, b, i, v);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -318,7 +336,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
   // ---- the four waves' results meet: 2 and 3 into 0 and 1, then 1 into 0
   l += xor_f(l, 16);
   l += xor_f(l, 32);
-  if constexpr (!QREG) __syncthreads();  // q in LDS is read no more
+  __syncthreads();  // q in LDS is read no more
   float *ml = lds + 2 * NT * 64 * 4;     // [2][2][64] behind the two waves' accumulators
   v4f *ov = reinterpret_cast<v4f *>(lds);
 #pragma unroll
@@ -367,69 +385,65 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
   });
 }
 
-// Joins the pieces of the rows whose keys were cut: one wave per (token, query head).  The pieces' weights come from
-// one read of all their maxima, a lane each (64 at a time); the accumulators are then read 8 pieces at a time.
+// Joins the pieces of the rows whose keys were cut: one workgroup per (token, query head).  head_dim/4 threads read one
+// piece's accumulator, 16 bytes each; the others take further pieces, 4 at a time each, and the groups' sums meet in
+// LDS.  A few rows have many pieces (32768 keys of one token: 32 heads, 30 to 128 pieces each), so four waves read
+// them side by side; with many rows one wave per row (two for head_dim above 256) does.
 template <bool PAGED>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, int head_dim, int shift) {
-  const int lane = threadIdx.x & 63;
+  __shared__ v4f sums[256];
+  __shared__ float group_l[16], group_m[4];
+  const int tid = threadIdx.x, lane = tid & 63;
   const unsigned heads = a.n_kv_heads * a.group;
-  const unsigned w = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= (unsigned)a.n_tokens * heads) return;
-  const int tok = (int)(w / heads), head = (int)(w - (w / heads) * heads);
-  const int hk = head / a.group, hr = head - hk * a.group;
-  int unit = 0;
+  const int tok = (int)(blockIdx.x / heads), head = (int)(blockIdx.x - tok * heads);
+  const int hk = head / a.group;
+  int hr = head - hk * a.group, unit = tok;
   AttnUnit u;
-  if (!attn_find<PAGED>(a, shift, unit, tok, hr, u) || u.pieces == 1) return;
+  if (!attn_find<PAGED, FIND_ROW>(a, shift, unit, hr, u) || u.pieces == 1) return;
   const int r = ((tok - u.s.q0) * a.group + hr) & ((1 << shift) - 1);
   // slot of piece p: the tile's row r in unit + p
   const long long slot0 = ((((long long)unit * a.n_kv_heads + hk) << shift) + r);
   const long long step = (long long)a.n_kv_heads << shift;
-  float m = -__builtin_inff(), l = 0.0f;
-  constexpr int NV = 8;  // head_dim <= 512
-  float o[NV] = {0, 0, 0, 0, 0, 0, 0, 0};
-  for (int p0 = 0; p0 < u.pieces; p0 += 64) {
-    float mp = -__builtin_inff(), lp = 0.0f;
-    if (p0 + lane < u.pieces) {
-      const float *ml = a.part_ml + (slot0 + (p0 + lane) * step) * 2;
-      mp = ml[0], lp = ml[1];
-    }
-    float top = mp;
-    for (int x = 32; x; x >>= 1) top = fmaxf(top, xor_f(top, x));
-    const float nm = fmaxf(m, top);
-    if (nm > -__builtin_inff()) {
-      const float alpha = __builtin_amdgcn_exp2f(m - nm);
-      l *= alpha;
+  float m = -__builtin_inff();
+  for (int p = tid; p < u.pieces; p += blockDim.x) m = fmaxf(m, a.part_ml[(slot0 + p * step) * 2]);
+  for (int x = 32; x; x >>= 1) m = fmaxf(m, xor_f(m, x));
+  if (tid < 4) group_m[tid] = -__builtin_inff();
+  __syncthreads();
+  if (lane == 0) group_m[tid >> 6] = m;
+  const int wide = head_dim / 4, groups = (int)blockDim.x / wide, grp = tid / wide, d = (tid - grp * wide) * 4;
+  __syncthreads();
+  m = fmaxf(fmaxf(group_m[0], group_m[1]), fmaxf(group_m[2], group_m[3]));
+  const float ref = m == -__builtin_inff() ? 0.0f : m;
+  v4f o = {0, 0, 0, 0};
+  float l = 0.0f;
+  if (grp < groups)
+    for (int p = grp; p < u.pieces; p += 4 * groups) {
+      v4f v[4];
+      float mp[4], lp[4];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) o[i] *= alpha;
-      m = nm;
-    }
-    const float ref = m == -__builtin_inff() ? 0.0f : m;
-    const float wgt = __builtin_amdgcn_exp2f(mp - ref);  // an empty piece: 2^-inf = 0
-    float sum = wgt * lp;
-    for (int x = 32; x; x >>= 1) sum += xor_f(sum, x);
-    l += sum;
-    const int n = u.pieces - p0 < 64 ? u.pieces - p0 : 64;
-    for (int p = 0; p < n; p += 8) {
-      float v[8][NV];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float *src = a.part_o + (slot0 + (p0 + (p + j < n ? p + j : n - 1)) * step) * head_dim;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) v[j][i] = lane + 64 * i < head_dim ? src[lane + 64 * i] : 0.0f;
+      for (int j = 0; j < 4; ++j) {
+        const long long s = slot0 + (p + j * groups < u.pieces ? p + j * groups : p) * step;
+        mp[j] = a.part_ml[s * 2], lp[j] = a.part_ml[s * 2 + 1];
+        v[j] = *reinterpret_cast<const v4f_a16 *>(a.part_o + s * head_dim + d);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float wj = p + j < n ? __shfl(wgt, p + j) : 0.0f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) o[i] += wj * v[j][i];
+      for (int j = 0; j < 4; ++j) {
+        // an empty piece weighs 2^-inf = 0
+        const float w = p + j * groups < u.pieces ? __builtin_amdgcn_exp2f(mp[j] - ref) : 0.0f;
+        l += w * lp[j];
+        o += w * v[j];
       }
     }
+  sums[tid] = o;
+  if (d == 0 && grp < groups) group_l[grp] = l;
+  __syncthreads();
+  if (grp != 0) return;
+  for (int g = 1; g < groups; ++g) {
+    o += sums[g * wide + tid];
+    l += group_l[g];
   }
   const float mul = l == 0.0f ? 0.0f : 1.0f / l;
-  float *dst = a.out + (long long)tok * a.out_stride + (long long)head * head_dim;
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (lane + 64 * i < head_dim) dst[lane + 64 * i] = o[i] * mul;
+  *reinterpret_cast<v4f_a16 *>(a.out + (long long)tok * a.out_stride + (long long)head * head_dim + d) = o * mul;
 }
 
 template <int D>
@@ -467,12 +481,12 @@ void launch_attention(const AttnArgs &a, int head_dim, bool paged, int shift, lo
       case 512: rows_launch<512>(a, paged, grid, stream); break;
     }
   if (split) {
-    const long long waves = (long long)a.n_tokens * a.n_kv_heads * a.group;
-    const unsigned blocks = (unsigned)((waves + 3) / 4);
+    const unsigned blocks = (unsigned)(a.n_tokens * a.n_kv_heads * a.group);
+    const dim3 threads(blocks <= 1024 ? 256 : (head_dim <= 256 ? 64 : 128));
     if (paged)
-      enqueue(attention_join_kernel<true>, dim3(blocks), dim3(256), 0, stream, a, head_dim, shift);
+      enqueue(attention_join_kernel<true>, dim3(blocks), threads, 0, stream, a, head_dim, shift);
     else
-      enqueue(attention_join_kernel<false>, dim3(blocks), dim3(256), 0, stream, a, head_dim, shift);
+      enqueue(attention_join_kernel<false>, dim3(blocks), threads, 0, stream, a, head_dim, shift);
   }
 }
 

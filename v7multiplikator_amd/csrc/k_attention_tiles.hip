@@ -53,12 +53,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
   constexpr int NL = (kKeys * CR + 255) / 256;  // 16-byte pieces of a K tile per thread
   constexpr auto pieces = std::make_integer_sequence<int, NL>{};
   extern __shared__ _Float16 tile_lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = lane >> 5, c = lane & 31;
-  const int hk = blockIdx.x % a.n_kv_heads;
-  int unit = blockIdx.x / a.n_kv_heads;
+  int hk, unit = blockIdx.x;
   AttnUnit u;
-  if (!attn_find<PAGED>(a, kAttnTileShift, unit, -1, 0, u)) return;
+  if (!attn_find<PAGED, FIND_HEADS_LAST>(a, kAttnTileShift, unit, hk, u)) return;
   const AttnSeq s = u.s;
   const int row0 = u.tile * kAttnTileRows + wave * 32;
   const int left = s.nq * a.group - row0;
@@ -121,7 +120,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
       for (int i = 0; i < 2; ++i) {
         pg[i] = -1;
         if (kb + 16 * i < key_hi) {
-          const int p = a.table[(long long)u.seq * a.table_width + ((kb + 16 * i) >> a.page_shift)];
+          const int p = page_entry(a.table, (long long)u.seq * a.table_width + ((kb + 16 * i) >> a.page_shift));
           pg[i] = (unsigned)p < (unsigned)a.n_pages ? p : -1;
         }
       }

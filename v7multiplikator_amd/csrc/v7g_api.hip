@@ -944,27 +944,40 @@ V7_ABI void v7s_rope_init(int head_dim, float rope_base) {
 namespace {
 
 // How a call is cut: tiles of rows, and pieces of their keys where the tiles alone leave compute units idle.
-// max_keys is the most keys a sequence can have, as far as the host knows.
+// max_keys is the most keys a sequence can have, as far as the host knows; self: causal over its own tokens.
 struct AttnPlan {
-  int shift = 0;  // tiles of 2^shift rows
+  int shift = 0;          // tiles of 2^shift rows
   int target = 0;         // units per KV head aimed at, 0: whole tiles
   long long units = 0;    // at most, per KV head
   long long workspace = 0;
 };
 
-AttnPlan attn_plan(int n_seqs, int n_tokens, int group, int n_kv_heads, int head_dim, long long max_keys) {
+AttnPlan attn_plan(int n_seqs, int n_tokens, int group, int n_kv_heads, int head_dim, long long max_keys, bool self) {
   AttnPlan p;
   const long long rows = (long long)n_tokens * group;
-  p.shift = head_dim <= v7g::kAttnTileDims && rows > 32LL * n_seqs ? v7g::kAttnTileShift : v7g::kAttnRowShift;
+  // 128-row tiles from 41 rows a sequence on (8 sequences of 4-5000 keys, 32/8 heads x 128, rows a sequence: 27 60 us
+  // in 16-row tiles against 76, 37 78 against 76, 53 94 against 79), wide heads from 97 on (x 256: 27 159 against 338,
+  // 73 309 against 314): there a compute unit holds one such workgroup, not two.
+  const bool many = head_dim <= v7g::kAttnTileDims && rows > (head_dim <= 128 ? 40LL : 96LL) * n_seqs;
+  p.shift = many ? v7g::kAttnTileShift : v7g::kAttnRowShift;
   const long long tiles = (rows >> p.shift) + n_seqs;
   p.units = tiles;
-  if (tiles * n_kv_heads < v7g::kAttnUnits && max_keys > v7g::kAttnMinChunk) {
-    p.target = (v7g::kAttnUnits + n_kv_heads - 1) / n_kv_heads;
+  // Units aimed at: four rounds of a workgroup per compute unit (6 trees of up to 60 drafts: 1024 units 116 us, 512
+  // 134, 2048 129; 37 decoded tokens 172, 185, 179), one round of the wide 128-row tiles (4 trees x 256: 256 units
+  // 248 us, 1024 306).  A prompt over its own keys is cut only if its tiles leave half of the chip idle: its longest
+  // tile is twice the mean, and joining costs as much as the tail (2048 tokens, 28/4 heads: whole 93 us, cut 128 to
+  // 180; 512 tokens, 32/8 heads: 29 against 36).
+  const int aim = many && head_dim > 128 ? v7g::kAttnUnits / 4 : v7g::kAttnUnits;
+  if (tiles * n_kv_heads < (self && many ? v7g::kAttnUnits / 8 : aim) && max_keys > v7g::kAttnMinChunk) {
+    p.target = (aim + n_kv_heads - 1) / n_kv_heads;
     p.units = tiles + p.target;
     p.workspace = ((p.units * n_kv_heads) << p.shift) * (head_dim + 2) * 4;
   }
   return p;
 }
+
+// Prompts that mostly see their own keys, not a long past.
+bool own_keys(int n_tokens, int n_kv_tokens) { return n_kv_tokens <= 4LL * n_tokens; }
 
 int check_attention(int n_seqs, int n_tokens, int n_q_heads, int n_kv_heads, int head_dim) {
   if (n_seqs < 0 || n_tokens < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0)
@@ -1019,7 +1032,8 @@ extern "C" {
 int64_t v7g_attention_prefill_workspace(int n_seqs, int n_tokens, int n_kv_tokens, int n_q_heads, int n_kv_heads,
                                         int head_dim) {
   if (check_attention(n_seqs, n_tokens, n_q_heads, n_kv_heads, head_dim)) return 0;
-  return attn_plan(n_seqs, n_tokens, n_q_heads / n_kv_heads, n_kv_heads, head_dim, n_kv_tokens).workspace;
+  return attn_plan(n_seqs, n_tokens, n_q_heads / n_kv_heads, n_kv_heads, head_dim, n_kv_tokens,
+                   own_keys(n_tokens, n_kv_tokens)).workspace;
 }
 
 int v7g_attention_prefill(float *out, long long out_stride, const float *q, long long q_stride, const uint16_t *k,
@@ -1033,7 +1047,8 @@ int v7g_attention_prefill(float *out, long long out_stride, const float *q, long
       bad_stride(k_stride, n_kv_tokens, krow) || bad_stride(v_stride, n_kv_tokens, krow))
     return fail(V7G_ERR_SHAPE);
   if (n_tokens == 0 || n_seqs == 0) return V7G_OK;
-  const AttnPlan p = attn_plan(n_seqs, n_tokens, n_q_heads / n_kv_heads, n_kv_heads, head_dim, n_kv_tokens);
+  const AttnPlan p = attn_plan(n_seqs, n_tokens, n_q_heads / n_kv_heads, n_kv_heads, head_dim, n_kv_tokens,
+                               own_keys(n_tokens, n_kv_tokens));
   if (!out || !q || !cu_seqlens || (n_kv_tokens > 0 && (!k || !v)) || (p.workspace && !workspace))
     return fail(V7G_ERR_NULL);
   if (workspace_bytes < p.workspace) return fail(V7G_ERR_SHAPE);
@@ -1063,8 +1078,8 @@ int v7g_attention_prefill(float *out, long long out_stride, const float *q, long
 int64_t v7g_attention_tree_workspace(int n_seqs, int n_tokens, int table_width, int page_size, int n_q_heads,
                                      int n_kv_heads, int head_dim) {
   if (table_width < 0 || page_size < 0 || check_attention(n_seqs, n_tokens, n_q_heads, n_kv_heads, head_dim)) return 0;
-  return attn_plan(n_seqs, n_tokens, n_q_heads / n_kv_heads, n_kv_heads, head_dim, (long long)table_width * page_size)
-      .workspace;
+  return attn_plan(n_seqs, n_tokens, n_q_heads / n_kv_heads, n_kv_heads, head_dim, (long long)table_width * page_size,
+                   false).workspace;
 }
 
 int v7g_attention_tree(float *out, long long out_stride, const float *q, long long q_stride,
@@ -1081,7 +1096,7 @@ int v7g_attention_tree(float *out, long long out_stride, const float *q, long lo
   if (tree_mask ? (mask_words <= 0 || mask_words >= (1 << 24)) : mask_words != 0) return fail(V7G_ERR_SHAPE);
   if (bad_stride(out_stride, n_tokens, qrow) || bad_stride(q_stride, n_tokens, qrow)) return fail(V7G_ERR_SHAPE);
   if (n_tokens == 0 || n_seqs == 0) return V7G_OK;
-  const AttnPlan p = attn_plan(n_seqs, n_tokens, n_q_heads / g.n_kv_heads, g.n_kv_heads, g.head_dim, cap);
+  const AttnPlan p = attn_plan(n_seqs, n_tokens, n_q_heads / g.n_kv_heads, g.n_kv_heads, g.head_dim, cap, false);
   // with no page or no table there is no key: every token of a sequence gives zeros
   const bool none = g.n_pages == 0 || table_width == 0;
   if (!out || !q || !context_lens || (!none && !block_table) || (p.workspace && !workspace)) return fail(V7G_ERR_NULL);

@@ -80,6 +80,13 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs &a, int b) {
   return s;
 }
 
+// An entry of the block table, the same for the whole wave: through the scalar cache, so that waiting for it does not
+// wait for the K and V rows on their way.
+__device__ __forceinline__ int page_entry(const int32_t *table, long long i) {
+  typedef const __attribute__((address_space(4))) int32_t *constant_p;
+  return ((constant_p)(uintptr_t)table)[i];
+}
+
 // A unit of work: a tile of rows of a sequence and one piece of its keys.
 struct AttnUnit {
   AttnSeq s;
@@ -103,13 +110,24 @@ __device__ __forceinline__ int attn_tiles(const AttnSeq &s, int group, int shift
   return (int)(((unsigned)(s.nq * group) + (1u << shift) - 1) >> shift);
 }
 
+// Sequence b of the step of 64 that starts at b0; the first step is kept by the caller.
+template <bool PAGED>
+__device__ __forceinline__ AttnSeq attn_step(const AttnArgs &a, int b0, const AttnSeq &first) {
+  AttnSeq s{0, 0, 0, 0, 0};
+  if (b0 == 0)
+    s = first;
+  else if (b0 + (int)__lane_id() < a.n_seqs)
+    s = attn_seq<PAGED>(a, b0 + __lane_id());
+  return s;
+}
+
 // Keys per piece: the summed key counts of all tiles over the units aimed at, in whole blocks of 64.  Every
 // workgroup derives the same number from the lengths, so the host needs none of them.
 template <bool PAGED>
-__device__ __forceinline__ int attn_piece_keys(const AttnArgs &a, int shift) {
+__device__ __forceinline__ int attn_piece_keys(const AttnArgs &a, int shift, const AttnSeq &first) {
   long long sum = 0;
-  for (int b = __lane_id(); b < a.n_seqs; b += 64) {
-    const AttnSeq s = attn_seq<PAGED>(a, b);
+  for (int b0 = 0; b0 < a.n_seqs; b0 += 64) {
+    const AttnSeq s = attn_step<PAGED>(a, b0, first);
     sum += (long long)attn_tiles(s, a.group, shift) * s.kv;
   }
   for (int m = 32; m; m >>= 1) sum += __shfl_xor(sum, m);
@@ -117,25 +135,43 @@ __device__ __forceinline__ int attn_piece_keys(const AttnArgs &a, int shift) {
   return keys < kAttnMinChunk ? kAttnMinChunk : (keys > 0x7fffff00 ? 0x7fffffff : ((int)keys + 63) & ~63);
 }
 
-// Unit number `want`; with of_token >= 0 instead the unit of row row_in_token of that token (its first piece), whose
-// number is returned in `want`.  False: past the last.  Every lane of the wave takes part.  Units go by sequences,
-// tiles from the last (which sees the most keys) to the first, and pieces; where nothing is cut and one step of the
-// wave's lanes holds all sequences, by tiles first, the longest of all sequences to the shortest.
-template <bool PAGED>
-__device__ __forceinline__ bool attn_find(const AttnArgs &a, int shift, int &want, int of_token, int row_in_token,
-                                          AttnUnit &u) {
-  u.piece_keys = a.split_target ? attn_piece_keys<PAGED>(a, shift) : 0x7fffffff;
+__device__ __forceinline__ int attn_pieces(const AttnSeq &s, int piece_keys) {
+  return s.kv <= piece_keys ? 1 : (int)(((unsigned)s.kv + (unsigned)piece_keys - 1) / (unsigned)piece_keys);
+}
+
+// What a workgroup does.  FIND_HEADS_LAST: `want` counts the KV heads fastest (workgroups that run together share a
+// head's K/V rows in one L2, as the compute dies are dealt workgroups in turn); FIND_HEADS_FIRST: it counts units
+// fastest, and comes back as the unit with the head in `hk`; FIND_ROW: the first piece's unit of row `hk` of token
+// `want`.  False: past the last.  Every lane of the wave takes part.  Units go by sequences, tiles from the last (which
+// sees the most keys) to the first, and pieces; where nothing is cut and one step of the wave's lanes holds all
+// sequences, by tiles first, the longest of all sequences to the shortest.
+enum { FIND_HEADS_LAST, FIND_HEADS_FIRST, FIND_ROW };
+
+template <bool PAGED, int MODE>
+__device__ __forceinline__ bool attn_find(const AttnArgs &a, int shift, int &want, int &hk, AttnUnit &u) {
   const int lane = __lane_id();
+  AttnSeq first{0, 0, 0, 0, 0};
+  if (lane < a.n_seqs) first = attn_seq<PAGED>(a, lane);
+  u.piece_keys = a.split_target ? attn_piece_keys<PAGED>(a, shift, first) : 0x7fffffff;
+  if constexpr (MODE == FIND_HEADS_LAST) {
+    hk = (unsigned)want % (unsigned)a.n_kv_heads;
+    want = (unsigned)want / (unsigned)a.n_kv_heads;
+  }
+  if constexpr (MODE == FIND_HEADS_FIRST) {
+    int total = 0;
+    for (int b0 = 0; b0 < a.n_seqs; b0 += 64) {
+      const AttnSeq s = attn_step<PAGED>(a, b0, first);
+      total += wave_sum(attn_tiles(s, a.group, shift) * attn_pieces(s, u.piece_keys));
+    }
+    if (total == 0) return false;
+    hk = (unsigned)want / (unsigned)total;
+    want -= hk * total;
+    if (hk >= a.n_kv_heads) return false;
+  }
   int base = 0;
   for (int b0 = 0; b0 < a.n_seqs; b0 += 64) {
-    const int b = b0 + lane;
-    AttnSeq s{0, 0, 0, 0, 0};
-    int tiles = 0, pieces = 1;
-    if (b < a.n_seqs) {
-      s = attn_seq<PAGED>(a, b);
-      tiles = attn_tiles(s, a.group, shift);
-      pieces = s.kv <= u.piece_keys ? 1 : (int)(((unsigned)s.kv + (unsigned)u.piece_keys - 1) / (unsigned)u.piece_keys);
-    }
+    const AttnSeq s = attn_step<PAGED>(a, b0, first);
+    const int tiles = attn_tiles(s, a.group, shift), pieces = attn_pieces(s, u.piece_keys);
     auto take = [&](int l) {
       u.seq = b0 + l;
       u.s.q0 = __builtin_amdgcn_readlane(s.q0, l);
@@ -145,7 +181,7 @@ __device__ __forceinline__ bool attn_find(const AttnArgs &a, int shift, int &wan
       u.s.off = __builtin_amdgcn_readlane(s.off, l);
       u.pieces = __builtin_amdgcn_readlane(pieces, l);
     };
-    if (!a.split_target && a.n_seqs > 1 && a.n_seqs <= 64) {
+    if (MODE != FIND_ROW && !a.split_target && a.n_seqs > 1 && a.n_seqs <= 64) {
       // from(t): the units of tiles t and later, which come before all others
       auto from = [&](int t) { return wave_sum(tiles > t ? tiles - t : 0); };
       if (want >= from(0)) return false;
@@ -172,22 +208,22 @@ __device__ __forceinline__ bool attn_find(const AttnArgs &a, int shift, int &wan
       const int o = __shfl_up(incl, d);
       if (lane >= d) incl += o;
     }
-    const bool mine = of_token >= 0 ? (of_token >= s.q0 && of_token < s.q0 + s.nq)
-                                    : (want >= base + incl - units && want < base + incl);
+    const bool mine = MODE == FIND_ROW ? (want >= s.q0 && want < s.q0 + s.nq)
+                                       : (want >= base + incl - units && want < base + incl);
     const unsigned long long hit = __ballot(mine);
     if (hit) {
       const int l = __builtin_ctzll(hit);
       take(l);
-      const int first = base + __builtin_amdgcn_readlane(incl - units, l);
+      const int begin = base + __builtin_amdgcn_readlane(incl - units, l);
       const int n = __builtin_amdgcn_readlane(tiles, l);
-      if (of_token >= 0) {
-        u.tile = ((of_token - u.s.q0) * a.group + row_in_token) >> shift;
+      if constexpr (MODE == FIND_ROW) {
+        u.tile = ((want - u.s.q0) * a.group + hk) >> shift;
         u.piece = 0;
-        want = first + (n - 1 - u.tile) * u.pieces;
+        want = begin + (n - 1 - u.tile) * u.pieces;
       } else {
-        const int t = (int)((unsigned)(want - first) / (unsigned)u.pieces);
+        const int t = (int)((unsigned)(want - begin) / (unsigned)u.pieces);
         u.tile = n - 1 - t;
-        u.piece = (want - first) - t * u.pieces;
+        u.piece = (want - begin) - t * u.pieces;
       }
       return true;
     }
