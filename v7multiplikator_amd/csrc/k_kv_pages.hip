@@ -46,51 +46,66 @@ __global__ __launch_bounds__(256) void kv_pack_pages_kernel(v7g_kv_pages g, cons
 
 // ---- accepted drafts moved to the front of their sequence's new tokens
 
+// Lane k's value, whichever lanes take part.
+__device__ __forceinline__ long long lane_value(long long v, int k) {
+  const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, k);
+  const unsigned hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(v >> 32), k);
+  return (long long)(((unsigned long long)hi << 32) | lo);
+}
+
 // Token i of row r's path goes from position len + path[i] to len + i.  A path is strictly ascending, so path[i] >= i
 // and moving it in order, 8 rows at a time (all 8 read before one is written), never overwrites a row that is still
-// to be read.  A workgroup takes one sequence, one layer, K or V, and 256 units of the row.
+// to be read.  A thread takes one unit of the row in one layer, K or V; where the rows lie is worked out once, a lane
+// per token of the path, and broadcast.  Bound by the latency of that chain of reads in the small cases.
 template <typename U>
 __global__ __launch_bounds__(256) void kv_compact_kernel(v7g_kv_pages g, const int32_t *table, int width,
                                                          const int32_t *lens, const int32_t *path, int path_width,
                                                          const int32_t *n_path, int32_t *lens_out, int page_shift,
                                                          int units) {
-  const int r = blockIdx.x, layer = blockIdx.y >> 1;
-  const int lane = threadIdx.x & 63;
+  const int r = blockIdx.x, lane = threadIdx.x & 63;
   const int32_t *tr = table + (long long)r * width, *p = path + (long long)r * path_width;
   const long long cap = (long long)width << page_shift;
-  const long long len = lens[r] < 0 ? 0 : (lens[r] > cap ? cap : lens[r]);
-  int want = n_path[r] < 0 ? 0 : (n_path[r] > path_width ? path_width : n_path[r]);
-  // the path ends at the first entry that does not ascend or has no page to come from or go to
+  const int given = n_path[r], ln = lens[r];
+  const long long len = ln < 0 ? 0 : (ln > cap ? cap : ln);
+  const int want = given < 0 ? 0 : (given > path_width ? path_width : given);
+  const unsigned at = blockIdx.y * 256u + threadIdx.x;  // layer, K or V, unit
+  const unsigned side = at / (unsigned)units;
+  const bool moves = side < 2u * g.n_layers;
+  constexpr int E = sizeof(U) / 2;
+  uint16_t *base = ((side & 1) ? g.v : g.k) + (moves ? (side >> 1) * g.layer_stride + (at - side * units) * E : 0);
   int n = 0;
   while (n < want) {
+    // the path ends at the first entry that does not ascend or has no page to come from or go to
     const int i = n + lane;
-    bool ok = false;
+    long long src = -1, dst = -1;
     if (i < want) {
       const int from = p[i], before = i ? p[i - 1] : -1;
-      ok = from > before && row_offset(g, page_shift, tr, width, len + from) >= 0 &&
-           row_offset(g, page_shift, tr, width, len + i) >= 0;
+      if (from > before) {
+        src = row_offset(g, page_shift, tr, width, len + from);
+        dst = row_offset(g, page_shift, tr, width, len + i);
+      }
     }
-    const unsigned long long good = __ballot(ok);
+    const unsigned long long good = __ballot(src >= 0 && dst >= 0);
     const int run = good == ~0ull ? 64 : __builtin_ctzll(~good);
     n += run;
+    if (moves)
+      for (int i0 = 0; i0 < run; i0 += 8) {
+        U v[8];
+        long long to[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int k = i0 + j < run ? i0 + j : i0;
+          const long long from = lane_value(src, k);
+          to[j] = lane_value(dst, k);
+          v[j] = *reinterpret_cast<const U *>(base + from);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (i0 + j < run) *reinterpret_cast<U *>(base + to[j]) = v[j];
+      }
     if (run < 64) break;
   }
-  if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) lens_out[r] = (int)(len + n);
-  const int u = blockIdx.z * 256 + threadIdx.x;
-  if (u >= units) return;
-  uint16_t *base = ((blockIdx.y & 1) ? g.v : g.k) + layer * g.layer_stride;
-  constexpr int E = sizeof(U) / 2;
-  for (int i0 = 0; i0 < n; i0 += 8) {
-    U v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i0 + i < n && p[i0 + i] != i0 + i)
-        v[i] = *reinterpret_cast<const U *>(base + row_offset(g, page_shift, tr, width, len + p[i0 + i]) + u * E);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i0 + i < n && p[i0 + i] != i0 + i)
-        *reinterpret_cast<U *>(base + row_offset(g, page_shift, tr, width, len + i0 + i) + u * E) = v[i];
-  }
+  if (blockIdx.y == 0 && threadIdx.x == 0) lens_out[r] = (int)(len + n);
 }
 
 // ---- sequences forked, freed and grown
@@ -102,6 +117,27 @@ struct AssignArgs {
   int rows, width, page_shift;
   int32_t *keep, *want, *tail;  // per row: pages kept, pages wanted, parent row whose last page is copied or -1
   int32_t *list;                // free pages found
+};
+
+// What row r takes over from row par, which holds `held` pages; owner: it takes over the last and spare ones too.
+struct AssignRow {
+  int n = 0, keep = 0, want = 0, tail = -1;
+  __device__ AssignRow() {}
+  __device__ AssignRow(const AssignArgs &a, int r, int par, int held, bool owner) {
+    const long long cap = (long long)held << a.page_shift;
+    const int ln = a.lens[par];
+    n = ln < 0 ? 0 : (ln > cap ? (int)cap : ln);
+    const int full = n >> a.page_shift, rest = n & ((1 << a.page_shift) - 1);
+    keep = owner ? held : full;
+    const long long more = a.reserve && a.reserve[r] > 0 ? a.reserve[r] : 0;
+    long long w = (n + more + (1 << a.page_shift) - 1) >> a.page_shift;
+    if (w > a.width) w = a.width;
+    want = (int)(w > keep ? w : keep);
+    if (!owner && rest) {
+      tail = par;
+      if (want < full + 1) want = full + 1;
+    }
+  }
 };
 
 __global__ __launch_bounds__(256) void assign_refs_kernel(AssignArgs a) {
@@ -135,13 +171,9 @@ __global__ __launch_bounds__(256) void assign_rows_kernel(AssignArgs a) {
   int par = a.parents[r];
   if (par < 0 || par >= a.rows) par = -1;
   const int held_r = pages_held(a, r, &scratch);
-  int keep = 0, want = 0, tail = -1, n = 0;
+  AssignRow row;
   if (par >= 0) {
     const int held = par == r ? held_r : pages_held(a, par, &scratch);
-    const long long cap = (long long)held << a.page_shift;
-    const int ln = a.lens[par];
-    n = ln < 0 ? 0 : (ln > cap ? (int)cap : ln);
-    const int full = n >> a.page_shift, rest = n & ((1 << a.page_shift) - 1);
     // the parent itself, else the lowest of its children, takes over the last and the spare pages
     bool owner = par == r;
     if (!owner) {
@@ -152,21 +184,13 @@ __global__ __launch_bounds__(256) void assign_rows_kernel(AssignArgs a) {
       __syncthreads();
       owner = scratch == 0;
     }
-    keep = owner ? held : full;
-    const long long more = a.reserve ? (a.reserve[r] > 0 ? a.reserve[r] : 0) : 0;
-    long long w = (n + more + (1 << a.page_shift) - 1) >> a.page_shift;
-    if (w > a.width) w = a.width;
-    want = (int)(w > keep ? w : keep);
-    if (!owner && rest) {
-      tail = par;
-      if (want < full + 1) want = full + 1;
-    }
+    row = AssignRow(a, r, par, held, owner);
   }
   const int32_t *mine = a.table + (long long)r * a.width;
   const int32_t *src = a.table + (long long)(par < 0 ? 0 : par) * a.width;
   int32_t *out = a.table_out + (long long)r * a.width;
   for (int i = threadIdx.x; i < a.width; i += 256) {
-    const int old = i < held_r ? mine[i] : -1, now = i < keep ? src[i] : -1;
+    const int old = i < held_r ? mine[i] : -1, now = i < row.keep ? src[i] : -1;
     out[i] = now;
     if (old != now) {
       if (old >= 0) atomicSub(a.refs_out + old, 1);
@@ -174,10 +198,10 @@ __global__ __launch_bounds__(256) void assign_rows_kernel(AssignArgs a) {
     }
   }
   if (threadIdx.x == 0) {
-    a.lens_out[r] = n;
-    a.keep[r] = keep;
-    a.want[r] = want;
-    a.tail[r] = tail;
+    a.lens_out[r] = row.n;
+    a.keep[r] = row.keep;
+    a.want[r] = row.want;
+    a.tail[r] = row.tail;
   }
 }
 
@@ -245,6 +269,109 @@ __global__ __launch_bounds__(1024) void assign_pages_kernel(AssignArgs a) {
   if (threadIdx.x == 0) *a.short_out = total - found;
 }
 
+// All of the above in one workgroup, the counts in LDS: where they fit, one launch and a few trips to memory instead
+// of three launches.
+constexpr int kBookPages = 24576, kBookRows = 1024, kBookEntries = 1 << 16;
+
+__global__ __launch_bounds__(1024) void assign_books_kernel(AssignArgs a) {
+  __shared__ int scratch[16];
+  extern __shared__ int lds[];
+  int *held = lds, *owner = held + a.rows, *keeps = owner + a.rows, *refs = keeps + a.rows;
+  const int tid = threadIdx.x, P = a.g.n_pages, W = a.width;
+  const int lane = tid & 63, wave = tid >> 6;
+  for (int p = tid; p < P; p += 1024) refs[p] = a.refs[p];
+  int par = -1;
+  if (tid < a.rows) {
+    par = a.parents[tid];
+    if (par >= a.rows || par < 0) par = -1;
+    owner[tid] = a.rows;
+  }
+  // a wave takes 4 rows at a time, their entries side by side in its lanes
+  constexpr int R = 4;
+  for (int r0 = wave * R; r0 < a.rows; r0 += 16 * R) {
+    int h[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) h[j] = W;
+    for (int c = 0; c < W; c += 64) {
+      int page[R];
+#pragma unroll
+      for (int j = 0; j < R; ++j)
+        page[j] = r0 + j < a.rows && c + lane < W ? a.table[(r0 + j) * W + c + lane] : 0;
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        const unsigned long long none = __ballot(c + lane < W && (unsigned)page[j] >= (unsigned)P);
+        if (none && h[j] == W) h[j] = c + __builtin_ctzll(none);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+      if (r0 + j < a.rows && lane == j) held[r0 + j] = h[j];
+  }
+  __syncthreads();
+  if (par >= 0) atomicMin(owner + par, par == tid ? -1 : tid);
+  __syncthreads();
+  AssignRow row;
+  if (par >= 0) row = AssignRow(a, tid, par, held[par], par == tid || owner[par] == tid);
+  __syncthreads();
+  if (tid < a.rows) {
+    keeps[tid] = row.keep;
+    owner[tid] = par;  // from here on, where the row's pages come from
+    a.keep[tid] = row.keep;
+    a.tail[tid] = row.tail;
+  }
+  __syncthreads();
+  for (int r0 = wave * R; r0 < a.rows; r0 += 16 * R)
+    for (int c = 0; c < W; c += 64) {
+      int old[R], now[R];
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        const int r = r0 + j, i = c + lane;
+        old[j] = now[j] = -1;
+        if (r < a.rows) {
+          if (i < held[r]) old[j] = a.table[r * W + i];
+          if (i < keeps[r]) now[j] = a.table[owner[r] * W + i];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        if (r0 + j < a.rows && c + lane < W) a.table_out[(r0 + j) * W + c + lane] = now[j];
+        if (old[j] != now[j]) {
+          if (old[j] >= 0) atomicSub(refs + old[j], 1);
+          if (now[j] >= 0) atomicAdd(refs + now[j], 1);
+        }
+      }
+    }
+  int total;
+  const int need = row.want - row.keep;
+  const int at = block_scan(need, scratch, total);  // its barriers end the counting too
+  int found = 0;
+  for (int p0 = 0; p0 < P && found < total; p0 += 16 * 1024) {
+    const int p = p0 + tid * 16;
+    unsigned bits = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (p + i < P && refs[p + i] <= 0) bits |= 1u << i;
+    int sum;
+    int to = found + block_scan(__builtin_popcount(bits), scratch, sum);
+    for (; bits; bits &= bits - 1, ++to)
+      if (to < total) a.list[to] = p + __builtin_ctz(bits);
+    found += sum;
+  }
+  if (found > total) found = total;
+  __threadfence_block();
+  __syncthreads();
+  for (int j = 0; j < need && at + j < found; ++j) {
+    const int page = a.list[at + j];
+    a.table_out[tid * a.width + row.keep + j] = page;
+    refs[page] = 1;
+  }
+  // no page for the copy of the last one: the row ends with its full pages
+  if (tid < a.rows) a.lens_out[tid] = row.tail >= 0 && at >= found ? row.keep << a.page_shift : row.n;
+  if (tid == 0) *a.short_out = total - found;
+  __syncthreads();
+  for (int p = tid; p < P; p += 1024) a.refs_out[p] = refs[p];
+}
+
 // The tokens of the last, partly filled page of a parent copied to its child's own page, in every layer.  The page
 // read is kept by the row that took it over, the page written is held by nobody else.
 template <typename U>
@@ -290,7 +417,7 @@ void launch_kv_compact(const v7g_kv_pages &g, const int32_t *table, int width, i
                        hipStream_t stream) {
   const bool wide = wide_rows(g);
   const int units = g.n_kv_heads * g.head_dim / (wide ? 8 : 4);
-  const dim3 grid((unsigned)rows, (unsigned)(2 * g.n_layers), (unsigned)((units + 255) / 256));
+  const dim3 grid((unsigned)rows, (unsigned)((2LL * g.n_layers * units + 255) / 256));
   const int shift = __builtin_ctz((unsigned)g.page_size);
   if (wide)
     enqueue(kv_compact_kernel<v4u>, grid, dim3(256), 0, stream, g, table, width, lens, path, path_width, n_path,
@@ -312,10 +439,14 @@ void launch_kv_assign(const v7g_kv_pages &g, int32_t *table_out, int32_t *lens_o
   a.want = a.keep + rows;
   a.tail = a.want + rows;
   a.list = a.tail + rows;
-  if (g.n_pages)
-    enqueue(assign_refs_kernel, dim3((unsigned)((g.n_pages + 255) / 256)), dim3(256), 0, stream, a);
-  if (rows) enqueue(assign_rows_kernel, dim3((unsigned)rows), dim3(256), 0, stream, a);
-  enqueue(assign_pages_kernel, dim3(1), dim3(1024), 0, stream, a);
+  if (g.n_pages <= kBookPages && rows <= kBookRows && (long long)rows * width <= kBookEntries) {
+    enqueue(assign_books_kernel, dim3(1), dim3(1024), (unsigned)(4 * (3 * rows + g.n_pages)), stream, a);
+  } else {
+    if (g.n_pages)
+      enqueue(assign_refs_kernel, dim3((unsigned)((g.n_pages + 255) / 256)), dim3(256), 0, stream, a);
+    if (rows) enqueue(assign_rows_kernel, dim3((unsigned)rows), dim3(256), 0, stream, a);
+    enqueue(assign_pages_kernel, dim3(1), dim3(1024), 0, stream, a);
+  }
   if (!rows || !g.n_pages) return;
   const bool wide = wide_rows(g);
   const int units = g.n_kv_heads * g.head_dim / (wide ? 8 : 4);

@@ -5,9 +5,10 @@
 // One pass over the logits, which is what bounds it: each lane keeps its own running maximum and sums (a new maximum
 // scales s and moves w: w' = a (w + s (m - m'))), and each wave the K best of what it has read.  A token is ordered by
 // one 64-bit key, the value's bits made monotonic above the complement of its index, so equal values fall to the
-// lower index, -0 equals 0 and NaN comes first.  A wave reads 1024 logits at a time; only keys above the K-th best so
-// far are looked at (until K are there: above the K-th best of the 64 lanes' best), collected in LDS and ranked by
-// counting.  A row goes to as many workgroups as fill the chip; a second kernel then joins their results.
+// lower index, -0 equals 0 and NaN comes first.  A wave reads 1024 logits at a time; those above a bar that K logits are
+// known to reach (first the K-th best of the 64 lanes' best) are collected in LDS, and ranked by counting, which
+// raises the bar, when 128 have come together and at the end.  A row goes to as many workgroups as fill the chip; a
+// second kernel then joins their results.
 #include "v7g_device.h"
 #include "v7g_internal.h"
 
@@ -17,6 +18,8 @@ namespace {
 
 constexpr int kChunk = 1024;  // logits of one step of a wave, 16 a lane
 constexpr int kBest = 64;     // at most so many alternatives
+constexpr int kRoom = 128;    // keys that wait to be ranked
+constexpr int kBuffer = kRoom + kChunk + 8 + kBest;  // a wave's keys: waiting, one step's, padding, the new list
 typedef unsigned long long Key;
 typedef float f4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -35,63 +38,102 @@ __device__ __forceinline__ int key_index(Key k) { return (int)(0xffffffffu - (ui
 
 __device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
-// The K-th largest of the lanes' keys: the largest key that K lanes reach, bit by bit.
+// The K-th largest of the lanes' keys: the largest that K lanes reach, bit by bit; the lower half only where values
+// tie.
 __device__ __forceinline__ Key kth_of_lanes(Key mine, int K) {
-  Key t = 0;
-  for (int b = 63; b >= 0; --b) {
-    const Key c = t | (1ull << b);
-    if (__popcll(__ballot(mine >= c)) >= K) t = c;
+  const uint32_t hi = (uint32_t)(mine >> 32);
+  uint32_t t = 0;
+  for (int b = 31; b >= 0; --b) {
+    const uint32_t c = t | (1u << b);
+    if (__popcll(__ballot(hi >= c)) >= K) t = c;
   }
-  return t;
+  Key key = (Key)t << 32;
+  if (__popcll(__ballot(hi >= t)) == K) return key;
+  for (int b = 31; b >= 0; --b) {
+    const Key c = key | (1ull << b);
+    if (__popcll(__ballot(mine >= c)) >= K) key = c;
+  }
+  return key;
 }
 
-// A wave's K best keys, sorted, at the front of its LDS buffer [kBest + kChunk + kBest]; the room behind takes the
-// candidates of one step and the new list.
+// A wave's best keys, in LDS: the K best of all it was given are among the n that wait there.
 struct Best {
   Key *buf;
   int K, n = 0;
-  Key worst = 0;  // the K-th key once there are K
+  float bar = -__builtin_inff();  // K keys with this value or a larger one are there (NaN counts as the largest)
+  bool full = false;              // the bar stands
+  bool sorted = false;
 
-  // Keys of one step, N a lane.
+  // The keys of `hit` lanes join the n that wait.
+  __device__ __forceinline__ void push(bool mine, Key k) {
+    const unsigned long long hit = __ballot(mine);
+    if (!hit) return;
+    if (mine)
+      buf[n + __builtin_amdgcn_mbcnt_hi((unsigned)(hit >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)hit, 0))] = k;
+    n += __popcll(hit);
+    sorted = false;
+  }
+
+  // Keys of one step, N a lane, 0 for none, in any order.
   template <int N>
   __device__ __forceinline__ void add(const Key (&k)[N]) {
     Key top = k[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) top = k[i] > top ? k[i] : top;
-    if (!__ballot(top > worst)) return;
-    Key bar = worst + 1;
-    if (n < K) {
-      const Key t = kth_of_lanes(top, K);
-      bar = t > 1 ? t : 1;
+    Key least = kth_of_lanes(top, K);
+    least = least > 1 ? least : 1;
+    if (full) {  // the keys that wait already hold the K best so far
+      const Key worst = sorted ? buf[K - 1] : 0;
+      least = worst + 1 > least ? worst + 1 : least;
     }
-    int cnt = n;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const unsigned long long hit = __ballot(k[i] >= bar);
-      if (hit) {
-        if (k[i] >= bar) buf[cnt + __builtin_amdgcn_mbcnt_hi((unsigned)(hit >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)hit, 0))] = k[i];
-        cnt += __popcll(hit);
-      }
-    }
-    rank(cnt);
+    for (int i = 0; i < N; ++i) push(k[i] >= least, k[i]);
+    settle();
   }
 
-  // The K best of the buffer's first cnt keys become the list.
-  __device__ __forceinline__ void rank(int cnt) {
-    Key *fresh = buf + kBest + kChunk;
+  // Values of one step in rising order of their indices, of which those above the bar count.
+  template <int N, class F>
+  __device__ __forceinline__ void add_above(const float (&v)[N], F key) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const bool mine = !(v[i] <= bar);  // NaN too
+      if (__ballot(mine)) push(mine, mine ? key(i) : 0);
+    }
+    settle();
+  }
+
+  __device__ __forceinline__ void settle() {
+    if (n > kRoom || (!full && n >= K)) rank();
+  }
+
+  // The K best of the n keys, sorted, to the front.
+  __device__ __forceinline__ void rank() {
+    Key *fresh = buf + kRoom + kChunk + 8;
+    const int lane = __lane_id();
+    if (lane < 8) buf[n + lane] = 0;  // read 8 at a time
     wave_lds_fence();
-    for (int i0 = 0; i0 < cnt; i0 += 64) {
-      const int i = i0 + __lane_id();
-      const Key mine = i < cnt ? buf[i] : 0;
+    for (int i0 = 0; i0 < n; i0 += 64) {
+      const int i = i0 + lane;
+      const Key mine = i < n ? buf[i] : 0;
       int r = 0;
-      for (int j = 0; j < cnt; ++j) r += buf[j] > mine;
-      if (i < cnt && r < K) fresh[r] = mine;
+      for (int j = 0; j < n; j += 8) {
+        Key o[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) o[x] = buf[j + x];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) r += o[x] > mine;
+      }
+      if (i < n && r < K) fresh[r] = mine;
     }
     wave_lds_fence();
-    n = cnt < K ? cnt : K;
-    if ((int)__lane_id() < n) buf[__lane_id()] = fresh[__lane_id()];
+    n = n < K ? n : K;
+    if (lane < n) buf[lane] = fresh[lane];
     wave_lds_fence();
-    if (n == K) worst = buf[K - 1];
+    sorted = true;
+    if (n == K) {
+      full = true;
+      bar = key_value(buf[K - 1]);
+    }
   }
 };
 
@@ -154,7 +196,7 @@ __device__ __forceinline__ void write_row(const LogprobArgs &a, long long row, c
 
 template <bool TOP>
 __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
-  __shared__ Key keys[TOP ? 4 : 1][TOP ? kBest + kChunk + kBest : 1];
+  __shared__ alignas(16) Key keys[TOP ? 4 : 1][TOP ? kBuffer : 1];
   __shared__ float sums[4][3];
   __shared__ int counts[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -195,18 +237,22 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
       t.w += e > 0.0f ? e * z : 0.0f;
     }
     if constexpr (TOP) {
-      Key k[16];
+      auto key = [&](int i) { return make_key(v[i], (unsigned)(at + (i >> 2) * 256 + (i & 3))); };
+      if (!best.full) {
+        Key k[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const long long q = at + (i >> 2) * 256 + (i & 3);
-        k[i] = q < a.vocab ? make_key(v[i], (unsigned)q) : 0;
+        for (int i = 0; i < 16; ++i) k[i] = at + (i >> 2) * 256 + (i & 3) < a.vocab ? key(i) : 0;
+        best.add(k);
+      } else if (__ballot(!(mx <= best.bar) || !(t.s == t.s))) {
+        best.add_above(v, key);
       }
-      best.add(k);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = nv[i];
   }
   t.join_lanes();
+  if constexpr (TOP)
+    if (!best.sorted) best.rank();
   if (lane == 0) {
     sums[wave][0] = t.m, sums[wave][1] = t.s, sums[wave][2] = t.w;
     counts[wave] = best.n;
@@ -215,13 +261,8 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
   if (wave != 0) return;
   for (int w = 1; w < 4; ++w) t.join(sums[w][0], sums[w][1], sums[w][2]);
   if constexpr (TOP) {
-    int cnt = best.n;
-    for (int w = 1; w < 4; ++w) {
-      const int n = counts[w];
-      if (lane < n) best.buf[cnt + lane] = keys[w][lane];
-      cnt += n;
-    }
-    best.rank(cnt);
+    for (int w = 1; w < 4; ++w) best.push(lane < counts[w], lane < counts[w] ? keys[w][lane] : 0);
+    best.rank();
   }
   if (a.parts == 1) {
     write_row(a, row, t, best.buf);
@@ -237,7 +278,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
 
 template <bool TOP>
 __global__ __launch_bounds__(64) void logprobs_join_kernel(LogprobArgs a) {
-  __shared__ Key keys[TOP ? kBest + kChunk + kBest : 1];
+  __shared__ alignas(16) Key keys[TOP ? kBuffer : 1];
   const int lane = threadIdx.x;
   const long long row = blockIdx.x;
   Sums t;
@@ -250,12 +291,13 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(LogprobArgs a) {
   if constexpr (TOP) {
     const Key *in = a.part_keys + row * a.parts * a.K;
     const int n = a.parts * a.K;
-    for (int i0 = 0; i0 < n; i0 += 64 * 8) {
-      Key k[8];
+    for (int i0 = 0; i0 < n; i0 += kChunk) {
+      Key k[16];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) k[i] = i0 + i * 64 + lane < n ? in[i0 + i * 64 + lane] : 0;
+      for (int i = 0; i < 16; ++i) k[i] = i0 + i * 64 + lane < n ? in[i0 + i * 64 + lane] : 0;
       best.add(k);
     }
+    if (!best.sorted) best.rank();
   }
   write_row(a, row, t, best.buf);
 }

@@ -968,7 +968,7 @@ AttnPlan attn_plan(int n_seqs, int n_tokens, int group, int n_kv_heads, int head
   // tile is twice the mean, and joining costs as much as the tail (2048 tokens, 28/4 heads: whole 93 us, cut 128 to
   // 180; 512 tokens, 32/8 heads: 29 against 36).
   const int aim = many && head_dim > 128 ? v7g::kAttnUnits / 4 : v7g::kAttnUnits;
-  if (tiles * n_kv_heads < (self && many ? v7g::kAttnUnits / 8 : aim) && max_keys > v7g::kAttnMinChunk) {
+  if (tiles * n_kv_heads < (self ? v7g::kAttnUnits / 8 : aim) && max_keys > v7g::kAttnMinChunk) {
     p.target = (aim + n_kv_heads - 1) / n_kv_heads;
     p.units = tiles + p.target;
     p.workspace = ((p.units * n_kv_heads) << p.shift) * (head_dim + 2) * 4;
@@ -1005,7 +1005,7 @@ int check_pages(const v7g_kv_pages &g) {
       (g.page_size & (g.page_size - 1)) || g.n_kv_heads <= 0 || g.head_dim <= 0)
     return V7G_ERR_SHAPE;
   const long long row = (long long)g.n_kv_heads * g.head_dim;
-  if (row % 4 || row >= (1LL << 24) || bad_stride(g.token_stride, g.page_size, row)) return V7G_ERR_SHAPE;
+  if (row % 4 || row >= (1LL << 24) || row * g.n_layers >= (1LL << 25) || bad_stride(g.token_stride, g.page_size, row)) return V7G_ERR_SHAPE;
   const long long page = (g.page_size - 1) * g.token_stride + row;
   if (g.page_stride % 4 || (g.n_pages > 1 && g.page_stride < page)) return V7G_ERR_SHAPE;
   const long long layer = (g.n_pages > 1 ? (g.n_pages - 1) * g.page_stride : 0) + page;

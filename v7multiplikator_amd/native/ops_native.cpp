@@ -15,6 +15,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <cstdint>
 #include <initializer_list>
 #include <limits>
@@ -41,6 +42,16 @@ struct Entries {
   decltype(&v7g_qkv_rope_stage) qkv_rope_stage;
   decltype(&v7g_kv_pack_f16) kv_pack_f16;
   decltype(&v7g_kv_pack_f16_kv) kv_pack_f16_kv;
+  decltype(&v7g_attention_prefill) attention_prefill;
+  decltype(&v7g_attention_prefill_workspace) attention_prefill_workspace;
+  decltype(&v7g_attention_tree) attention_tree;
+  decltype(&v7g_attention_tree_workspace) attention_tree_workspace;
+  decltype(&v7g_kv_pack_f16_pages) kv_pack_f16_pages;
+  decltype(&v7g_kv_pages_assign) kv_pages_assign;
+  decltype(&v7g_kv_pages_assign_workspace) kv_pages_assign_workspace;
+  decltype(&v7g_kv_pages_compact) kv_pages_compact;
+  decltype(&v7g_token_logprobs) token_logprobs;
+  decltype(&v7g_token_logprobs_workspace) token_logprobs_workspace;
 } lib;
 PyObject *raw_stream = nullptr;      // torch's raw current-stream query (device index -> stream handle)
 PyObject *current_device = nullptr;  // torch's raw current-device query
@@ -519,6 +530,204 @@ PyObject *kv_pack_f16_kv(const Call &c) {  // k_src, v_src, k_out, v_out
   return wrap2(ko, vo);
 }
 
+// ------------------------------------------------------------------ around the K/V cache
+
+// One call's scratch, from torch's allocator as ops takes it.
+struct Scratch {
+  at::Tensor t;
+  int64_t bytes;
+  Scratch(int64_t n, const at::Tensor &like) : bytes(n) {
+    if (n) t = without_gil([&] { return at::empty({n}, at::TensorOptions().device(like.device()).dtype(at::kByte)); });
+  }
+  void *ptr() const { return bytes ? t.data_ptr() : nullptr; }
+};
+
+int32_t *i32(const at::Tensor &t) { return static_cast<int32_t *>(t.data_ptr()); }
+
+at::Tensor fresh(const at::Tensor &like, at::IntArrayRef sizes, at::ScalarType type) {
+  return without_gil([&] { return at::empty(sizes, at::TensorOptions().device(like.device()).dtype(type)); });
+}
+
+// int32, one dimension; n < 0: of any length.
+const at::Tensor &ints(const Call &c, int i, int64_t n) {
+  const at::Tensor &t = c.t(i, at::kInt);
+  need(t.dim() == 1 && (n < 0 || t.numel() == n));
+  return t;
+}
+const at::Tensor &int_table(const Call &c, int i, int64_t rows) {
+  const at::Tensor &t = c.t(i, at::kInt);
+  need(t.dim() == 2 && (rows < 0 || t.size(0) == rows));
+  return t;
+}
+
+// v7g_kv_pages of [n_pages, page_size, heads, head_dim], or with layers in front.
+v7g_kv_pages kv_pages(const Call &c, int ik, int iv, bool layered) {
+  const at::Tensor &k = c.t(ik, at::kHalf, false), &v = c.t(iv, at::kHalf, false);
+  const int64_t n = k.dim();
+  need((n == 4 || (layered && n == 5)) && v.sizes() == k.sizes() && v.strides() == k.strides());
+  need(k.stride(n - 1) == 1 && (k.size(n - 2) <= 1 || k.stride(n - 2) == k.size(n - 1)));
+  v7g_kv_pages g = {};
+  g.k = f16(k);
+  g.v = f16(v);
+  g.n_layers = n == 5 ? dim32(k.size(0)) : 1;
+  g.layer_stride = n == 5 ? k.stride(0) : 0;
+  g.n_pages = dim32(k.size(n - 4));
+  g.page_size = dim32(k.size(n - 3));
+  g.n_kv_heads = dim32(k.size(n - 2));
+  g.head_dim = dim32(k.size(n - 1));
+  g.page_stride = k.stride(n - 4);
+  g.token_stride = k.stride(n - 3);
+  return g;
+}
+
+float score_scale(const Call &c, int i, int head_dim) {
+  if (!c.none(i)) return c.number(i);
+  need(head_dim > 0);
+  return static_cast<float>(1.0 / std::sqrt(static_cast<double>(head_dim)));
+}
+
+at::Tensor heads_out(const Call &c, int i, const at::Tensor &q, const Heads &h) {
+  if (c.none(i)) return fresh(q, {h.tokens, h.heads, h.hd}, at::kFloat);
+  const at::Tensor &o = c.t(i, at::kFloat, false);
+  need(Heads(o).same(h));
+  return o;
+}
+
+PyObject *wrap4(const at::Tensor &a, const at::Tensor &b, const at::Tensor &d, const at::Tensor &e) {
+  PyObject *r = PyTuple_New(4);
+  if (!r) throw Raised{};
+  const at::Tensor *ts[4] = {&a, &b, &d, &e};
+  for (int i = 0; i < 4; ++i) {
+    PyObject *o = THPVariable_Wrap(*ts[i]);
+    if (!o) {
+      Py_DECREF(r);
+      throw Raised{};
+    }
+    PyTuple_SET_ITEM(r, i, o);
+  }
+  return r;
+}
+
+PyObject *attention_prefill(const Call &c) {  // q, k, v, cu_seqlens, cu_seqlens_k, scale, out
+  const at::Tensor &q = c.t(0, at::kFloat, false), &k = c.t(1, at::kHalf, false), &v = c.t(2, at::kHalf, false);
+  const Heads hq(q), hk(k), hv(v);
+  need(hv.same(hk) && hk.hd == hq.hd);
+  const at::Tensor &cu = ints(c, 3, -1);
+  need(cu.numel() >= 1);
+  const int32_t *cuk = c.none(4) ? nullptr : i32(ints(c, 4, cu.numel()));
+  const int n_seqs = dim32(cu.numel() - 1);
+  const float scale = score_scale(c, 5, hq.hd);
+  const at::Tensor o = heads_out(c, 6, q, hq);
+  const Scratch ws(lib.attention_prefill_workspace(n_seqs, hq.tokens, hk.tokens, hq.heads, hk.heads, hq.hd), q);
+  c.bind();
+  launch("attention_prefill", [&] {
+    return lib.attention_prefill(f32(o), o.stride(0), f32(q), hq.stride, f16(k), hk.stride, f16(v), hv.stride, i32(cu),
+                                 cuk, n_seqs, hq.tokens, hk.tokens, hq.heads, hk.heads, hq.hd, scale, ws.ptr(),
+                                 ws.bytes);
+  });
+  return c.none(6) ? wrap(o) : same(c.a[6]);
+}
+
+// q, k_pages, v_pages, block_table, context_lens, cu_seqlens, tree_mask, scale, out
+PyObject *attention_tree(const Call &c) {
+  const at::Tensor &q = c.t(0, at::kFloat, false);
+  const Heads hq(q);
+  const v7g_kv_pages g = kv_pages(c, 1, 2, false);
+  need(g.head_dim == hq.hd);
+  const at::Tensor &lens = ints(c, 4, -1);
+  const int n_seqs = dim32(lens.numel());
+  const at::Tensor &table = int_table(c, 3, n_seqs);
+  const int width = dim32(table.size(1));
+  const int32_t *cu = c.none(5) ? nullptr : i32(ints(c, 5, static_cast<int64_t>(n_seqs) + 1));
+  need(cu || hq.tokens == n_seqs);
+  const int64_t *mask = nullptr;
+  int words = 0;
+  if (!c.none(6)) {
+    const at::Tensor &m = c.t(6, at::kLong);
+    need((m.dim() == 1 || m.dim() == 2) && m.size(0) == hq.tokens && hq.tokens > 0);
+    words = m.dim() == 2 ? dim32(m.size(1)) : 1;
+    need(words > 0);
+    mask = static_cast<const int64_t *>(m.data_ptr());
+  }
+  const float scale = score_scale(c, 7, hq.hd);
+  const at::Tensor o = heads_out(c, 8, q, hq);
+  const Scratch ws(
+      lib.attention_tree_workspace(n_seqs, hq.tokens, width, g.page_size, hq.heads, g.n_kv_heads, hq.hd), q);
+  c.bind();
+  launch("attention_tree", [&] {
+    return lib.attention_tree(f32(o), o.stride(0), f32(q), hq.stride, &g, i32(table), width, i32(lens), cu, mask, words,
+                              n_seqs, hq.tokens, hq.heads, scale, ws.ptr(), ws.bytes);
+  });
+  return c.none(8) ? wrap(o) : same(c.a[8]);
+}
+
+PyObject *kv_pack_f16_pages(const Call &c) {  // k_src, v_src, k_pages, v_pages, block_table, positions, seqs
+  const at::Tensor &k = rows_view(c, 0, at::kFloat), &v = rows_view(c, 1, at::kFloat);
+  need(v.sizes() == k.sizes() && v.strides() == k.strides());
+  const v7g_kv_pages g = kv_pages(c, 2, 3, false);
+  const int tokens = dim32(k.size(0));
+  need(k.size(1) == static_cast<int64_t>(g.n_kv_heads) * g.head_dim);
+  const at::Tensor &table = int_table(c, 4, -1);
+  const int n_seqs = dim32(table.size(0)), width = dim32(table.size(1));
+  const int32_t *pos = i32(ints(c, 5, tokens));
+  const int32_t *seqs = c.none(6) ? nullptr : i32(ints(c, 6, tokens));
+  need(seqs || tokens <= n_seqs);
+  c.bind();
+  launch("kv_pack_f16_pages", [&] {
+    return lib.kv_pack_f16_pages(&g, f32(k), f32(v), k.stride(0), i32(table), width, n_seqs, pos, seqs, tokens);
+  });
+  return same(Py_True);
+}
+
+PyObject *kv_pages_assign(const Call &c) {  // k_pages, v_pages, block_table, lens, refs, parents, reserve
+  const v7g_kv_pages g = kv_pages(c, 0, 1, true);
+  const at::Tensor &table = int_table(c, 2, -1);
+  const int n_seqs = dim32(table.size(0)), width = dim32(table.size(1));
+  const at::Tensor &lens = ints(c, 3, n_seqs), &refs = ints(c, 4, g.n_pages);
+  const int32_t *parents = i32(ints(c, 5, n_seqs));
+  const int32_t *reserve = c.none(6) ? nullptr : i32(ints(c, 6, n_seqs));
+  const at::Tensor to = fresh(refs, table.sizes(), at::kInt), lo = fresh(refs, lens.sizes(), at::kInt),
+                   ro = fresh(refs, refs.sizes(), at::kInt), so = fresh(refs, {1}, at::kInt);
+  const Scratch ws(lib.kv_pages_assign_workspace(n_seqs, g.n_pages), refs);
+  c.bind();
+  launch("kv_pages_assign", [&] {
+    return lib.kv_pages_assign(&g, i32(to), i32(lo), i32(ro), i32(so), i32(table), i32(lens), i32(refs), parents,
+                               reserve, n_seqs, width, ws.ptr(), ws.bytes);
+  });
+  return wrap4(to, lo, ro, so);
+}
+
+PyObject *kv_pages_compact(const Call &c) {  // k_pages, v_pages, block_table, lens, path, n_path
+  const v7g_kv_pages g = kv_pages(c, 0, 1, true);
+  const at::Tensor &table = int_table(c, 2, -1);
+  const int n_seqs = dim32(table.size(0)), width = dim32(table.size(1));
+  const at::Tensor &lens = ints(c, 3, n_seqs), &path = int_table(c, 4, n_seqs), &n_path = ints(c, 5, n_seqs);
+  const at::Tensor o = fresh(lens, lens.sizes(), at::kInt);
+  c.bind();
+  launch("kv_pages_compact", [&] {
+    return lib.kv_pages_compact(&g, i32(o), i32(table), width, i32(lens), i32(path), dim32(path.size(1)), i32(n_path),
+                                n_seqs);
+  });
+  return wrap(o);
+}
+
+PyObject *token_logprobs(const Call &c) {  // logits, ids, top_k
+  const at::Tensor &x = c.t(0, at::kFloat, false);
+  need(x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1));
+  const int tokens = dim32(x.size(0)), vocab = dim32(x.size(1)), top = c.integer(2, 0);
+  need(top <= 64);
+  const at::Tensor &ids = ints(c, 1, tokens);
+  const at::Tensor lp = fresh(x, {tokens}, at::kFloat), ent = fresh(x, {tokens}, at::kFloat),
+                   tl = fresh(x, {tokens, top}, at::kFloat), ti = fresh(x, {tokens, top}, at::kInt);
+  const Scratch ws(lib.token_logprobs_workspace(tokens, vocab, top), x);
+  c.bind();
+  launch("token_logprobs", [&] {
+    return lib.token_logprobs(f32(lp), f32(ent), top ? f32(tl) : nullptr, top ? i32(ti) : nullptr, f32(x), x.stride(0),
+                              i32(ids), tokens, vocab, top, ws.ptr(), ws.bytes);
+  });
+  return wrap4(lp, ent, tl, ti);
+}
+
 // Python entry: None where the call is not for this path.  No C++ exception leaves it.
 template <PyObject *(*F)(const Call &), int N>
 PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
@@ -565,6 +774,16 @@ PyObject *bind(PyObject *, PyObject *args) {
   V7G_ENTRY(qkv_rope_stage, "v7g_qkv_rope_stage")
   V7G_ENTRY(kv_pack_f16, "v7g_kv_pack_f16")
   V7G_ENTRY(kv_pack_f16_kv, "v7g_kv_pack_f16_kv")
+  V7G_ENTRY(attention_prefill, "v7g_attention_prefill")
+  V7G_ENTRY(attention_prefill_workspace, "v7g_attention_prefill_workspace")
+  V7G_ENTRY(attention_tree, "v7g_attention_tree")
+  V7G_ENTRY(attention_tree_workspace, "v7g_attention_tree_workspace")
+  V7G_ENTRY(kv_pack_f16_pages, "v7g_kv_pack_f16_pages")
+  V7G_ENTRY(kv_pages_assign, "v7g_kv_pages_assign")
+  V7G_ENTRY(kv_pages_assign_workspace, "v7g_kv_pages_assign_workspace")
+  V7G_ENTRY(kv_pages_compact, "v7g_kv_pages_compact")
+  V7G_ENTRY(token_logprobs, "v7g_token_logprobs")
+  V7G_ENTRY(token_logprobs_workspace, "v7g_token_logprobs_workspace")
 #undef V7G_ENTRY
   lib = e;
   Py_INCREF(s);
@@ -594,6 +813,12 @@ PyMethodDef methods[] = {{"bind", &bind, METH_VARARGS, nullptr},
                          V7G_OP(qkv_rope_stage, 17),
                          V7G_OP(kv_pack_f16, 2),
                          V7G_OP(kv_pack_f16_kv, 4),
+                         V7G_OP(attention_prefill, 7),
+                         V7G_OP(attention_tree, 9),
+                         V7G_OP(kv_pack_f16_pages, 7),
+                         V7G_OP(kv_pages_assign, 7),
+                         V7G_OP(kv_pages_compact, 6),
+                         V7G_OP(token_logprobs, 3),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -589,6 +589,9 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
     device; None: the same as cu_seqlens); its token i of n sees its first i + 1 + m - n rows of m.  scale defaults
     to 1/sqrt(D).  A token that sees nothing gives zeros; tokens of out behind the last sequence are left as they
     were."""
+    r = _fast.attention_prefill(q, k, v, cu_seqlens, cu_seqlens_k, scale, out)
+    if r is not None:
+        return r
     _need(q, torch.float32, "q", contiguous=False)
     T, Hq, D, qs = _heads_view(q, "q")
     for t, n in ((k, "k"), (v, "v")):
@@ -666,6 +669,9 @@ def attention_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     cu_seqlens[b] .. cu_seqlens[b+1]-1 (None: one each, T == B).  A new token sees the context and the new tokens up
     to itself, or, with tree_mask (int64, [T] or [T, words]), the new tokens j of its sequence whose bit j%64 of word
     j/64 is set.  Everything else as attention_prefill."""
+    r = _fast.attention_tree(q, k_pages, v_pages, block_table, context_lens, cu_seqlens, tree_mask, scale, out)
+    if r is not None:
+        return r
     _need(q, torch.float32, "q", contiguous=False)
     T, Hq, D, qs = _heads_view(q, "q")
     g = _kv_pages(k_pages, v_pages, False)
@@ -710,6 +716,8 @@ def kv_pack_f16_pages(k_src: torch.Tensor, v_src: torch.Tensor, k_pages: torch.T
     one layer's pages [n_pages, page_size, Hk, D]: token t's at position positions[t] of the sequence of block table
     row seqs[t] (None: row t).  A token with no such row, position or page is skipped; the places of one call are
     distinct."""
+    if _fast.kv_pack_f16_pages(k_src, v_src, k_pages, v_pages, block_table, positions, seqs):
+        return
     _need(k_src, torch.float32, "k_src", contiguous=False)
     _need(v_src, torch.float32, "v_src", contiguous=False)
     if k_src.dim() != 2 or k_src.stride(1) != 1 or v_src.shape != k_src.shape or v_src.stride() != k_src.stride():
@@ -741,6 +749,9 @@ def kv_pages_assign(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: t
     the one that takes it over (the parent itself, else its lowest fork).  New pages are the lowest free ones, in the
     order of the rows; short [1] counts those that were missing, whose entries stay -1 (a fork without its copy ends
     with its full pages).  All indices int32."""
+    r = _fast.kv_pages_assign(k_pages, v_pages, block_table, lens, refs, parents, reserve)
+    if r is not None:
+        return r
     g = _kv_pages(k_pages, v_pages, True)
     _table(block_table, None)
     B, W = block_table.shape
@@ -766,6 +777,9 @@ def kv_pages_compact(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: 
     """Keeps accepted drafts: of the new tokens behind lens[r] tokens of row r, those numbered path[r, :n_path[r]]
     (strictly ascending; the path ends at the first entry that does not ascend or has no page) move to the places from
     lens[r] on, in every layer of k_pages, v_pages [(layers,) n_pages, page_size, Hk, D].  Returns the new lens."""
+    r = _fast.kv_pages_compact(k_pages, v_pages, block_table, lens, path, n_path)
+    if r is not None:
+        return r
     g = _kv_pages(k_pages, v_pages, True)
     _table(block_table, None)
     B, W = block_table.shape
@@ -785,6 +799,9 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0):
     [T] in nats, top log probabilities [T, top_k], top ids [T, top_k] int32; top_k <= 64).  Equal logits: the lower
     index first.  An id outside the vocabulary gives NaN, a row with NaN or +inf or nothing above -inf NaN for every
     probability."""
+    r = _fast.token_logprobs(logits, ids, top_k)
+    if r is not None:
+        return r
     _need(logits, torch.float32, "logits", contiguous=False)
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits must be [tokens, vocab] with contiguous rows")
