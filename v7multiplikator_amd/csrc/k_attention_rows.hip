@@ -78,8 +78,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
   const bool tree = PAGED && a.mask_words;
   const int64_t *words = a.mask + (long long)(s.q0 + tok) * a.mask_words;
   // keys below lim are seen by the row, keys from lim on by the mask's bits or not at all
-  const int lim = tree ? min(s.off, s.kv) : clampi(s.off + tok + 1, 0, s.kv);
-  const int lim_min = tree ? lim : clampi(s.off + row0 / a.group + 1, 0, s.kv);
+  const int ctx = min(s.off, s.kv);
+  const int lim = tree ? ctx : clampi(s.off + tok + 1, 0, s.kv);
+  const int lim_min = tree ? ctx : clampi(s.off + row0 / a.group + 1, 0, s.kv);
   const int lim_max = tree ? s.kv : clampi(s.off + (row0 + n_rows - 1) / a.group + 1, 0, s.kv);
   const int key_lo = u.piece ? u.piece * u.piece_keys : 0;
   const int key_hi = u.piece + 1 < u.pieces ? min((u.piece + 1) * u.piece_keys, lim_max) : lim_max;

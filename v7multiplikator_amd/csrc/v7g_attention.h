@@ -93,7 +93,8 @@ struct AttnUnit {
   int seq, tile, piece, pieces, piece_keys;
 };
 
-// Sum over the wave's lanes, in every lane.
+// Sum over the wave's lanes.  Handed back through a scalar register, as every number here that all lanes share: the
+// compiler then keeps what follows from it (pages, row addresses, loop bounds) out of the vector registers.
 __device__ __forceinline__ int wave_sum(int v) {
   v += (int)dpp_u<DPP_QUAD_XOR1>((uint32_t)v);
   v += (int)dpp_u<DPP_QUAD_XOR2>((uint32_t)v);
@@ -102,7 +103,7 @@ __device__ __forceinline__ int wave_sum(int v) {
   const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
   v = (int)(a[0] + a[1]);
   const auto b = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
-  return (int)(b[0] + b[1]);
+  return __builtin_amdgcn_readfirstlane((int)(b[0] + b[1]));
 }
 
 // Tiles of 2^shift rows that a sequence has (tokens times heads stay below 2^31, the entry's check).
@@ -132,7 +133,8 @@ __device__ __forceinline__ int attn_piece_keys(const AttnArgs &a, int shift, con
   }
   for (int m = 32; m; m >>= 1) sum += __shfl_xor(sum, m);
   const long long keys = sum / a.split_target + 1;
-  return keys < kAttnMinChunk ? kAttnMinChunk : (keys > 0x7fffff00 ? 0x7fffffff : ((int)keys + 63) & ~63);
+  return __builtin_amdgcn_readfirstlane(
+      keys < kAttnMinChunk ? kAttnMinChunk : (keys > 0x7fffff00 ? 0x7fffffff : ((int)keys + 63) & ~63));
 }
 
 __device__ __forceinline__ int attn_pieces(const AttnSeq &s, int piece_keys) {
