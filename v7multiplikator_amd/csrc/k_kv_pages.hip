@@ -38,8 +38,8 @@ __global__ __launch_bounds__(256) void kv_pack_pages_kernel(v7g_kv_pages g, cons
   for (int j = threadIdx.x - sub * chunks; j < chunks; j += 256) {
     const float4 k = ld_stream4(k_src + t * src_stride + 4 * j);
     const float4 v = ld_stream4(v_src + t * src_stride + 4 * j);
-    *reinterpret_cast<uint2 *>(g.k + off + 4 * j) = pack4_f16(k);
-    *reinterpret_cast<uint2 *>(g.v + off + 4 * j) = pack4_f16(v);
+    st_stream_u2(reinterpret_cast<uint32_t *>(g.k + off + 4 * j), pack4_f16(k));
+    st_stream_u2(reinterpret_cast<uint32_t *>(g.v + off + 4 * j), pack4_f16(v));
     if (rows_per_wg > 1) break;
   }
 }
