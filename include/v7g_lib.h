@@ -463,9 +463,11 @@ int v7g_embedding_gather_q8(float *out, const int32_t *ids, int n_tokens, const 
  * n_kv_heads heads of head_dim elements, contiguous, at
  * k + l*layer_stride + p*page_stride + i*token_stride (v the same).  page_size
  * is a power of two, 16..65536; strides in elements, multiples of 4; k and v
- * 8-byte aligned.  A block table row [table_width] names the pages of a
+ * 8-byte aligned, apart from each other; n_layers * n_kv_heads * head_dim <
+ * 2^24.  A block table row [table_width] names the pages of a
  * sequence's tokens in order, page_size tokens each; an entry outside
- * [0, n_pages) is no page. */
+ * [0, n_pages) is no page.  A table's entries, and table_width * page_size,
+ * stay below 2^31, its rows and a call's tokens below 2^24. */
 typedef struct v7g_kv_pages {
     uint16_t *k, *v;
     int n_layers, n_pages, page_size, n_kv_heads, head_dim;
@@ -484,7 +486,8 @@ typedef struct v7g_kv_pages {
  * gives it NaN or infinity.
  * q, out: head_dim contiguous heads per token, token strides in floats, % 4;
  * k, v the same in binary16 elements, 8-byte aligned.  head_dim % 32 == 0 in
- * [64, 512]; n_q_heads a multiple of n_kv_heads.  out overlaps nothing.
+ * [64, 512]; n_q_heads a multiple of n_kv_heads; n_tokens * n_q_heads < 2^25
+ * and n_seqs * n_kv_heads below about 2^23.  out overlaps nothing.
  * workspace: v7g_attention_prefill_workspace(...) bytes (may be 0), 16-byte
  * aligned; its contents are not kept from call to call, and calls that may run
  * at the same time need their own. */

@@ -129,6 +129,40 @@ def test_prefill_offsets_out_of_range_stay_inside(ops):
     assert (out[40:] == 3.0).all() and torch.isfinite(out).all()
 
 
+def test_offsets_that_do_not_rise_stay_inside(ops):
+    """Sequences that overlap hold more tiles than the call has tokens for: what the scratch has no room for is left
+    out, of either kernel, whole or cut in pieces."""
+    g = gen(10)
+    for T, S, n in ((40, 3000, 30), (600, 9000, 20), (64, 64, 50), (2000, 2000, 9)):
+        q, k, v = rnd(g, T, 8, 64), rnd(g, S, 2, 64, dtype=torch.float16), rnd(g, S, 2, 64, dtype=torch.float16)
+        back = [0, T] * n
+        keys = [0, S] * n
+        out = torch.full((T + 64, 8, 64), 3.0, device="cuda")
+        ops.attention_prefill(q, k, v, i32(back + [0]), i32(keys + [0]), out=out[:T])
+        torch.cuda.synchronize()
+        assert (out[T:] == 3.0).all() and not torch.isnan(out).any()
+    kp, vp, table, ks, vs = paged(g, [3000, 100], 64, 2, 64)
+    table = table[:1].repeat(60, 1).contiguous()
+    kp, vp = torch.nan_to_num(kp), torch.nan_to_num(vp)
+    out = torch.full((100, 8, 64), 3.0, device="cuda")
+    for T in (10, 70):
+        ops.attention_tree(rnd(g, T, 8, 64), kp, vp, table, i32([2000] * 60), i32([0, T] * 30 + [0]), out=out[:T])
+        torch.cuda.synchronize()
+        assert (out[T:] == 3.0).all() and not torch.isnan(out).any()
+
+
+def test_subnormal_rows(ops):
+    """binary16 subnormals in K and V count as what they are."""
+    g = gen(12)
+    for n in (9, 300):
+        q = rnd(g, n, 4, 128, sigma=3e4)
+        k = rnd(g, n, 2, 128, sigma=1.5e-5, dtype=torch.float16)
+        v = rnd(g, n, 2, 128, sigma=4e-6, dtype=torch.float16)
+        out = ops.attention_prefill(q, k, v, cu([n]))
+        want, bound = R.attend(q, k, v, R.causal(n, n))
+        R.check(out, want, bound)
+
+
 def test_prefill_past_32_bit_offsets(ops):
     """K/V rows and tokens whose element offsets pass 2^31 and 2^32."""
     g = gen(11)

@@ -39,7 +39,7 @@ PREFILL = dict(out=at(0), out_stride=512, q=at(1), q_stride=512, k=at(2), k_stri
     (dict(n_seqs=-1), SHAPE), (dict(T=-1), SHAPE), (dict(S=-1, cuk=at(6)), SHAPE), (dict(S=599), SHAPE),
     (dict(Hq=7), SHAPE), (dict(Hq=0), SHAPE), (dict(Hk=0), SHAPE), (dict(D=48), SHAPE), (dict(D=32), SHAPE),
     (dict(D=544), SHAPE), (dict(q_stride=510), SHAPE), (dict(q_stride=508), SHAPE), (dict(out_stride=500), SHAPE),
-    (dict(k_stride=126), SHAPE), (dict(v_stride=124), SHAPE), (dict(T=1 << 29, S=1 << 29), SHAPE),
+    (dict(k_stride=126), SHAPE), (dict(v_stride=124), SHAPE), (dict(T=1 << 22, S=1 << 22), SHAPE), (dict(n_seqs=1 << 22), SHAPE),
     (dict(out=None), NULL), (dict(q=None), NULL), (dict(k=None), NULL), (dict(v=None), NULL), (dict(cu=None), NULL),
     (dict(out=at(0) + 4), ALIGN), (dict(q=at(1) + 8), ALIGN), (dict(k=at(2) + 4), ALIGN), (dict(v=at(3) + 2), ALIGN),
     (dict(cu=at(4) + 1), ALIGN), (dict(cuk=at(6) + 2), ALIGN),
@@ -86,7 +86,8 @@ def pages(**c):
 
 
 BAD_PAGES = [
-    (dict(n_layers=0), SHAPE), (dict(n_layers=20000), SHAPE), (dict(n_pages=-1), SHAPE), (dict(page_size=8), SHAPE),
+    (dict(n_layers=0), SHAPE), (dict(n_layers=20000), SHAPE),
+    (dict(n_layers=1 << 14, n_kv_heads=16, token_stride=1024, page_stride=16384, layer_stride=100 * 16384), SHAPE), (dict(n_pages=-1), SHAPE), (dict(page_size=8), SHAPE),
     (dict(page_size=24), SHAPE), (dict(page_size=1 << 17), SHAPE), (dict(n_kv_heads=0), SHAPE), (dict(head_dim=-64), SHAPE),
     (dict(token_stride=126), SHAPE), (dict(token_stride=124), SHAPE), (dict(page_stride=2044), SHAPE),
     (dict(page_stride=2046), SHAPE), (dict(n_layers=2, layer_stride=100 * 2048 - 4), SHAPE), (dict(layer_stride=2), SHAPE),
@@ -205,7 +206,7 @@ LOGPROBS = dict(lp=at(0), ent=at(1), tl=at(2), ti=at(3), x=at(4), stride=5000, i
 
 
 @pytest.mark.parametrize("c,want", [
-    (dict(T=-1), SHAPE), (dict(V=0), SHAPE), (dict(V=(1 << 30) + 1), SHAPE), (dict(K=-1), SHAPE), (dict(K=65), SHAPE),
+    (dict(T=-1), SHAPE), (dict(T=1 << 24), SHAPE), (dict(V=0), SHAPE), (dict(V=(1 << 30) + 1), SHAPE), (dict(K=-1), SHAPE), (dict(K=65), SHAPE),
     (dict(V=3), SHAPE), (dict(stride=4999), SHAPE), (dict(ws_bytes=8), SHAPE), (dict(lp=None), NULL), (dict(ent=None), NULL),
     (dict(tl=None), NULL), (dict(ti=None), NULL), (dict(x=None), NULL), (dict(ids=None), NULL), (dict(ws=None), NULL),
     (dict(lp=at(0) + 2), ALIGN), (dict(ent=at(1) + 1), ALIGN), (dict(tl=at(2) + 2), ALIGN), (dict(ti=at(3) + 2), ALIGN),

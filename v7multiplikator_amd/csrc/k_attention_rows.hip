@@ -68,7 +68,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
   // other order, 64 of 1000-4000 keys 158 -> 148)
   int hk, unit = blockIdx.x;
   AttnUnit u;
-  if (!attn_find<PAGED, FIND_HEADS_FIRST>(a, kAttnRowShift, unit, hk, u)) return;
+  if (!attn_find<PAGED, FIND_HEADS_FIRST>(a, kAttnRowShift, unit, hk, u) || unit >= a.units) return;
   const AttnSeq s = u.s;
   const int rows = s.nq * a.group, row0 = u.tile * 16;
   const int n_rows = rows - row0 < 16 ? rows - row0 : 16;
@@ -401,6 +401,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, int hea
   int hr = head - hk * a.group, unit = tok;
   AttnUnit u;
   if (!attn_find<PAGED, FIND_ROW>(a, shift, unit, hr, u) || u.pieces == 1) return;
+  if (unit > a.units - u.pieces) return;  // offsets that do not rise: sequences overlap, and some have no room
   const int r = ((tok - u.s.q0) * a.group + hr) & ((1 << shift) - 1);
   // slot of piece p: the tile's row r in unit + p
   const long long slot0 = ((((long long)unit * a.n_kv_heads + hk) << shift) + r);

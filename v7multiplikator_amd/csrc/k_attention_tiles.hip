@@ -63,7 +63,7 @@ __global__ __launch_bounds__(PAIR ? 512 : 256, D <= 128 ? 2 : 1) void attention_
   const int h = lane >> 5, c = lane & 31;
   int hk, unit = blockIdx.x;
   AttnUnit u;
-  if (!attn_find<PAGED, FIND_HEADS_LAST>(a, kAttnTileShift, unit, hk, u)) return;
+  if (!attn_find<PAGED, FIND_HEADS_LAST>(a, kAttnTileShift, unit, hk, u) || unit >= a.units) return;
   const AttnSeq s = u.s;
   const int row0 = u.tile * kAttnTileRows + wave * 32;
   const int left = s.nq * a.group - row0;

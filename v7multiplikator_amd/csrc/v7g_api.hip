@@ -983,9 +983,10 @@ int check_attention(int n_seqs, int n_tokens, int n_q_heads, int n_kv_heads, int
   if (n_seqs < 0 || n_tokens < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0)
     return V7G_ERR_SHAPE;
   if (head_dim < 64 || head_dim > 512 || head_dim % 32 != 0) return V7G_ERR_SHAPE;
-  if ((long long)n_tokens * n_q_heads >= (1LL << 31) - 64 || n_seqs >= (1 << 30)) return V7G_ERR_SHAPE;
+  // one workgroup per (token, head) or unit and KV head: both grids stay below 2^32 threads
+  if ((long long)n_tokens * n_q_heads >= (1LL << 25)) return V7G_ERR_SHAPE;
   const long long tiles = ((long long)n_tokens * (n_q_heads / n_kv_heads) >> v7g::kAttnRowShift) + n_seqs;
-  return (tiles + v7g::kAttnUnits) * n_kv_heads >= (1LL << 31) ? V7G_ERR_SHAPE : V7G_OK;
+  return (tiles + v7g::kAttnUnits) * n_kv_heads >= (1LL << 23) ? V7G_ERR_SHAPE : V7G_OK;
 }
 
 bool bad_stride(long long stride, long long rows, long long row_len) {
@@ -994,6 +995,7 @@ bool bad_stride(long long stride, long long rows, long long row_len) {
 
 int launch_attn(v7g::AttnArgs &a, const AttnPlan &p, int head_dim, bool paged, void *workspace) {
   a.split_target = p.target;
+  a.units = (int)p.units;
   a.part_o = static_cast<float *>(workspace);
   a.part_ml = a.part_o ? a.part_o + ((p.units * a.n_kv_heads) << p.shift) * head_dim : nullptr;
   v7g::launch_attention(a, head_dim, paged, p.shift, p.units, p.target != 0, stream());
@@ -1005,7 +1007,7 @@ int check_pages(const v7g_kv_pages &g) {
       (g.page_size & (g.page_size - 1)) || g.n_kv_heads <= 0 || g.head_dim <= 0)
     return V7G_ERR_SHAPE;
   const long long row = (long long)g.n_kv_heads * g.head_dim;
-  if (row % 4 || row >= (1LL << 24) || row * g.n_layers >= (1LL << 25) || bad_stride(g.token_stride, g.page_size, row)) return V7G_ERR_SHAPE;
+  if (row % 4 || row >= (1LL << 24) || row * g.n_layers >= (1LL << 24) || bad_stride(g.token_stride, g.page_size, row)) return V7G_ERR_SHAPE;
   const long long page = (g.page_size - 1) * g.token_stride + row;
   if (g.page_stride % 4 || (g.n_pages > 1 && g.page_stride < page)) return V7G_ERR_SHAPE;
   const long long layer = (g.n_pages > 1 ? (g.n_pages - 1) * g.page_stride : 0) + page;
@@ -1130,7 +1132,7 @@ int v7g_attention_tree(float *out, long long out_stride, const float *q, long lo
 
 // Block tables are indexed in 32 bits, and a sequence's positions too.
 static bool bad_table(const v7g_kv_pages &g, int n_seqs, int table_width) {
-  return n_seqs < 0 || table_width < 0 || (long long)table_width * g.page_size >= (1LL << 31) - 64 ||
+  return n_seqs < 0 || n_seqs >= (1 << 24) || table_width < 0 || (long long)table_width * g.page_size >= (1LL << 31) - 64 ||
          (long long)n_seqs * table_width >= (1LL << 31);
 }
 
@@ -1141,7 +1143,8 @@ int v7g_kv_pack_f16_pages(const v7g_kv_pages *pages, const float *k_src, const f
   const v7g_kv_pages &g = *pages;
   if (int rc = check_pages(g)) return fail(rc);
   const long long row = (long long)g.n_kv_heads * g.head_dim;
-  if (n_tokens < 0 || bad_table(g, n_seqs, table_width) || bad_stride(src_stride, n_tokens, row))
+  if (n_tokens < 0 || n_tokens >= (1 << 24) || bad_table(g, n_seqs, table_width) ||
+      bad_stride(src_stride, n_tokens, row))
     return fail(V7G_ERR_SHAPE);
   if (!seqs && n_tokens > n_seqs) return fail(V7G_ERR_SHAPE);
   if (n_tokens == 0 || n_seqs == 0 || table_width == 0 || g.n_pages == 0) return V7G_OK;
@@ -1229,7 +1232,7 @@ int64_t v7g_token_logprobs_workspace(int n_tokens, int vocab, int top_k) {
 int v7g_token_logprobs(float *logprob, float *entropy, float *top_logprob, int32_t *top_ids, const float *logits,
                        long long stride, const int32_t *ids, int n_tokens, int vocab, int top_k, void *workspace,
                        int64_t workspace_bytes) {
-  if (n_tokens < 0 || vocab <= 0 || vocab > (1 << 30) || top_k < 0 || top_k > 64 || top_k > vocab)
+  if (n_tokens < 0 || n_tokens >= (1 << 24) || vocab <= 0 || vocab > (1 << 30) || top_k < 0 || top_k > 64 || top_k > vocab)
     return fail(V7G_ERR_SHAPE);
   if (n_tokens > 1 && stride < vocab) return fail(V7G_ERR_SHAPE);
   if (n_tokens == 0) return V7G_OK;

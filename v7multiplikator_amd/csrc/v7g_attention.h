@@ -31,6 +31,7 @@ struct AttnArgs {
   int n_kv_heads, group;
   float scale_log2;  // the score scale times log2(e)
   int split_target;  // units per KV head aimed at; 0: no tile is split along the keys
+  int units;         // per KV head, at most: what the grid and the partial results have room for
   float *part_o;     // [unit, KV head, tile row, head_dim]
   float *part_ml;    // [unit, KV head, tile row, 2]: running maximum (log2 domain) and sum
 };
