@@ -463,7 +463,8 @@ int v7g_embedding_gather_q8(float *out, const int32_t *ids, int n_tokens, const 
  * n_kv_heads heads of head_dim elements, contiguous, at
  * k + l*layer_stride + p*page_stride + i*token_stride (v the same).  page_size
  * is a power of two, 16..65536; strides in elements, multiples of 4; k and v
- * 8-byte aligned, apart from each other; n_layers * n_kv_heads * head_dim <
+ * 8-byte aligned, apart from each other; each stride covers what it steps
+ * over (tokens within pages within layers); n_layers * n_kv_heads * head_dim <
  * 2^24.  A block table row [table_width] names the pages of a
  * sequence's tokens in order, page_size tokens each; an entry outside
  * [0, n_pages) is no page.  A table's entries, and table_width * page_size,

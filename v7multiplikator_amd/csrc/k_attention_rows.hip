@@ -86,34 +86,6 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
   const int key_hi = u.piece + 1 < u.pieces ? min((u.piece + 1) * u.piece_keys, lim_max) : lim_max;
   const int full_hi = min(key_hi, lim_min);  // up to here every row sees every key
 
-  // ---- q rows, scaled by a power of two and split in two binary16 parts; in LDS, where all four waves read them
-  v8h *qlds = reinterpret_cast<v8h *>(lds);  // [KS][2][64]
-  float factor;
-  {
-    const float *qr = a.q + (long long)(s.q0 + tok) * a.q_stride + (long long)head * D + g * 8;
-    float mx = 0.0f;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, __builtin_fabsf(qr[ks * 32 + i]));
-    mx = fmaxf(mx, xor_f(mx, 16));
-    mx = fmaxf(mx, xor_f(mx, 32));
-    const int e = q_row_exponent(mx);
-    factor = __builtin_ldexpf(a.scale_log2, -e);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-      if (ks % 4 == wave) {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __builtin_ldexpf(qr[ks * 32 + i], e);
-        v8h hi, lo;
-        split8(x, hi, lo);
-        qlds[(ks * 2) * 64 + lane] = hi;
-        qlds[(ks * 2 + 1) * 64 + lane] = lo;
-      }
-    __syncthreads();
-  }
-
   v4f acc[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) acc[t] = v4f{0, 0, 0, 0};
@@ -180,6 +152,48 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
       load_slice<W>(r + S::base(i) + c * W, v[j]);
     }
   };
+  constexpr auto whole = std::false_type{};
+  constexpr auto cut = std::true_type{};
+  auto load = [&](int kb, Rows &r) {
+    const Block b = block_at(kb);
+    r.ok[0] = b.ok[0], r.ok[1] = b.ok[1];
+    load_k(whole, b, r.k);
+    if constexpr (AHEAD) each(slices, [&](auto i) { load_v(whole, b, i, r.v[i]); });
+  };
+  // the first block is on its way while q is prepared
+  int kb = key_lo + wave * 32;
+  Rows ra;
+  if constexpr (AHEAD)
+    if (kb + 32 <= full_hi) load(kb, ra);
+
+  // ---- q rows, scaled by a power of two and split in two binary16 parts; in LDS, where all four waves read them
+  v8h *qlds = reinterpret_cast<v8h *>(lds);  // [KS][2][64]
+  float factor;
+  {
+    const float *qr = a.q + (long long)(s.q0 + tok) * a.q_stride + (long long)head * D + g * 8;
+    float mx = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, __builtin_fabsf(qr[ks * 32 + i]));
+    mx = fmaxf(mx, xor_f(mx, 16));
+    mx = fmaxf(mx, xor_f(mx, 32));
+    const int e = q_row_exponent(mx);
+    factor = __builtin_ldexpf(a.scale_log2, -e);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      if (ks % 4 == wave) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __builtin_ldexpf(qr[ks * 32 + i], e);
+        v8h hi, lo;
+        split8(x, hi, lo);
+        qlds[(ks * 2) * 64 + lane] = hi;
+        qlds[(ks * 2 + 1) * 64 + lane] = lo;
+      }
+    __syncthreads();
+  }
+
   auto scores = [&](const v4u (&k)[2][KS], v4f (&sc)[2]) {
     sc[0] = sc[1] = v4f{0, 0, 0, 0};
 #pragma unroll
@@ -226,15 +240,6 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
     }
   };
 
-  // ---- blocks whose keys every row sees
-  constexpr auto whole = std::false_type{};
-  constexpr auto cut = std::true_type{};
-  auto load = [&](int kb, Rows &r) {
-    const Block b = block_at(kb);
-    r.ok[0] = b.ok[0], r.ok[1] = b.ok[1];
-    load_k(whole, b, r.k);
-    if constexpr (AHEAD) each(slices, [&](auto i) { load_v(whole, b, i, r.v[i]); });
-  };
   auto compute = [&](int kb, Rows &r) {
     v4f sc[2];
     scores(r.k, sc);
@@ -261,10 +266,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
       add_slice(i, v);
     });
   };
-  int kb = key_lo + wave * 32;
+  // ---- blocks whose keys every row sees
   if constexpr (AHEAD) {
-    Rows ra, rb;
-    if (kb + 32 <= full_hi) load(kb, ra);
+    Rows rb;
     while (kb + 32 <= full_hi) {
       const bool second = kb + 160 <= full_hi;
       if (second) load(kb + 128, rb);
@@ -401,7 +405,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, int hea
   int hr = head - hk * a.group, unit = tok;
   AttnUnit u;
   if (!attn_find<PAGED, FIND_ROW>(a, shift, unit, hr, u) || u.pieces == 1) return;
-  if (unit > a.units - u.pieces) return;  // offsets that do not rise: sequences overlap, and some have no room
+  if (unit < 0 || unit > a.units - u.pieces) return;  // offsets that do not rise: sequences overlap, and some have no room
   const int r = ((tok - u.s.q0) * a.group + hr) & ((1 << shift) - 1);
   // slot of piece p: the tile's row r in unit + p
   const long long slot0 = ((((long long)unit * a.n_kv_heads + hk) << shift) + r);

@@ -83,36 +83,6 @@ __global__ __launch_bounds__(PAIR ? 512 : 256, D <= 128 ? 2 : 1) void attention_
   const int key_lo = u.piece ? u.piece * u.piece_keys : 0;
   const int key_hi = u.piece + 1 < u.pieces ? min((u.piece + 1) * u.piece_keys, tile_max) : tile_max;
 
-  // ---- q rows in two binary16 parts; the scale's sign goes with them, so that the largest product is the maximum
-  v8h qh[KS], ql[L::q_low ? 1 : KS];
-  v8h *qlow = reinterpret_cast<v8h *>(tile_lds + 2 * L::side) + wave * KS * 64 + lane;
-  float factor;
-  {
-    const float *qr = a.q + (long long)(s.q0 + tok) * a.q_stride + (long long)head * D + h * 8;
-    const float sign = a.scale_log2 < 0.0f ? -1.0f : (a.scale_log2 == 0.0f ? 0.0f : 1.0f);
-    float mx = 0.0f;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, __builtin_fabsf(qr[ks * 16 + i]));
-    mx = max_halves(mx);
-    const int e = q_row_exponent(mx);
-    // never 0: it multiplies the -inf of hidden keys (a factor this small makes every score vanish all the same)
-    factor = sign == 0.0f ? 1.0f : fmaxf(__builtin_ldexpf(__builtin_fabsf(a.scale_log2), -e), 0x1p-126f);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __builtin_ldexpf(qr[ks * 16 + i], e) * sign;
-      v8h low;
-      split8(x, qh[ks], low);
-      if constexpr (L::q_low)
-        qlow[ks * 64] = low;
-      else
-        ql[ks] = low;
-    }
-  }
-
   v16f acc[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) acc[t] = v16f{};
@@ -192,6 +162,47 @@ __global__ __launch_bounds__(PAIR ? 512 : 256, D <= 128 ? 2 : 1) void attention_
     });
   };
 
+  // the first step's rows are on their way while q is prepared
+  int pg[2] = {0, 0};
+  auto gone_of = [&] { return PAGED ? (pg[0] < 0 ? 1u : 0u) | (pg[1] < 0 ? 2u : 0u) : 0u; };
+  int kb = key_lo + group * kKeys;
+  unsigned gone = 0, next_gone = 0;
+  if (kb < key_hi) {
+    pages_at(kb, pg);
+    gone = gone_of();
+    fetch(kb, pg);
+  }
+
+  // ---- q rows in two binary16 parts; the scale's sign goes with them, so that the largest product is the maximum
+  v8h qh[KS], ql[L::q_low ? 1 : KS];
+  v8h *qlow = reinterpret_cast<v8h *>(tile_lds + 2 * L::side) + wave * KS * 64 + lane;
+  float factor;
+  {
+    const float *qr = a.q + (long long)(s.q0 + tok) * a.q_stride + (long long)head * D + h * 8;
+    const float sign = a.scale_log2 < 0.0f ? -1.0f : (a.scale_log2 == 0.0f ? 0.0f : 1.0f);
+    float mx = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, __builtin_fabsf(qr[ks * 16 + i]));
+    mx = max_halves(mx);
+    const int e = q_row_exponent(mx);
+    // never 0: it multiplies the -inf of hidden keys (a factor this small makes every score vanish all the same)
+    factor = sign == 0.0f ? 1.0f : fmaxf(__builtin_ldexpf(__builtin_fabsf(a.scale_log2), -e), 0x1p-126f);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = __builtin_ldexpf(qr[ks * 16 + i], e) * sign;
+      v8h low;
+      split8(x, qh[ks], low);
+      if constexpr (L::q_low)
+        qlow[ks * 64] = low;
+      else
+        ql[ks] = low;
+    }
+  }
+
   // One step on a buffer; bit i of gone: its keys 16i.. are on no page.  CUT: the mask, the piece's end or the last key
   // runs through it.
   auto step = [&](auto cut, const _Float16 *buf, int kb, unsigned gone) {
@@ -270,16 +281,7 @@ __global__ __launch_bounds__(PAIR ? 512 : 256, D <= 128 ? 2 : 1) void attention_
 
   // ---- the keys, 32 at a time: while one buffer is read, the other is filled and the step after fetched
   if (key_lo < key_hi) {
-    int pg[2] = {0, 0};
-    auto gone_of = [&] { return PAGED ? (pg[0] < 0 ? 1u : 0u) | (pg[1] < 0 ? 2u : 0u) : 0u; };
-    int kb = key_lo + group * kKeys;
-    unsigned gone = 0, next_gone = 0;
-    if (kb < key_hi) {
-      pages_at(kb, pg);
-      gone = gone_of();
-      fetch(kb, pg);
-      store(tile_lds);
-    }
+    if (kb < key_hi) store(tile_lds);
     if (kb + kStride < key_hi) {
       pages_at(kb + kStride, pg);
       next_gone = gone_of();

@@ -132,7 +132,10 @@ __device__ __forceinline__ int attn_piece_keys(const AttnArgs &a, int shift, con
     const AttnSeq s = attn_step<PAGED>(a, b0, first);
     sum += (long long)attn_tiles(s, a.group, shift) * s.kv;
   }
-  for (int m = 32; m; m >>= 1) sum += __shfl_xor(sum, m);
+  // 24 bits at a time through the fast lane sums
+  long long all = 0;
+  for (int i = 0; i < 3; ++i) all += (long long)wave_sum((int)(sum >> (24 * i)) & 0xffffff) << (24 * i);
+  sum = all;
   const long long keys = sum / a.split_target + 1;
   return __builtin_amdgcn_readfirstlane(
       keys < kAttnMinChunk ? kAttnMinChunk : (keys > 0x7fffff00 ? 0x7fffffff : ((int)keys + 63) & ~63));
@@ -227,6 +230,8 @@ __device__ __forceinline__ bool attn_find(const AttnArgs &a, int shift, int &wan
         const int t = (int)((unsigned)(want - begin) / (unsigned)u.pieces);
         u.tile = n - 1 - t;
         u.piece = (want - begin) - t * u.pieces;
+        // offsets that do not rise can add up past 32 bits: no tile then, rather than one of no sequence
+        if ((unsigned)t >= (unsigned)n) return false;
       }
       return true;
     }
