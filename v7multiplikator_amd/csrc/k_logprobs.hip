@@ -201,6 +201,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
   __shared__ alignas(16) Key keys[TOP ? 4 : 1][TOP ? kBuffer : 1];
   __shared__ float sums[4][3];
   __shared__ int counts[4];
+  __shared__ Key joined[TOP ? kBest : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long long row = blockIdx.x / a.parts;
   const int part = blockIdx.x % a.parts;
@@ -260,14 +261,34 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
     counts[wave] = best.n;
   }
   __syncthreads();
+  int n = 0;  // the waves' lists together
+  if constexpr (TOP) {
+    // a key's place is its place in its own list and those of the larger ones in the other three, by bisection
+    const Key mine = lane < best.n ? best.buf[lane] : 0;
+    int place = lane;
+    for (int o = 1; o < 4; ++o) {
+      const int w = (wave + o) & 3;
+      int lo = 0, hi = counts[w];
+      while (__ballot(lo < hi)) {
+        const int mid = (lo + hi) >> 1;
+        const bool larger = lo < hi && keys[w][mid] > mine;
+        if (lo < hi) {
+          if (larger)
+            lo = mid + 1;
+          else
+            hi = mid;
+        }
+      }
+      place += lo;
+    }
+    if (lane < best.n && place < a.K) joined[place] = mine;
+    n = counts[0] + counts[1] + counts[2] + counts[3];
+    __syncthreads();
+  }
   if (wave != 0) return;
   for (int w = 1; w < 4; ++w) t.join(sums[w][0], sums[w][1], sums[w][2]);
-  if constexpr (TOP) {
-    for (int w = 1; w < 4; ++w) best.push(lane < counts[w], lane < counts[w] ? keys[w][lane] : 0);
-    best.rank();
-  }
   if (a.parts == 1) {
-    write_row(a, row, t, best.buf);
+    write_row(a, row, t, joined);
     return;
   }
   const long long slot = row * a.parts + part;
@@ -275,7 +296,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
     float *p = a.part_sums + slot * 4;
     p[0] = t.m, p[1] = t.s, p[2] = t.w;
   }
-  if (TOP && lane < a.K) a.part_keys[slot * a.K + lane] = lane < best.n ? best.buf[lane] : 0;
+  if (TOP && lane < a.K) a.part_keys[slot * a.K + lane] = lane < n ? joined[lane] : 0;
 }
 
 template <bool TOP>
