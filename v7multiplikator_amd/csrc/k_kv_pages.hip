@@ -349,8 +349,10 @@ __global__ __launch_bounds__(1024) void assign_books_kernel(AssignArgs a) {
     const int p = p0 + tid * 16;
     unsigned bits = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (p + i < P && refs[p + i] <= 0) bits |= 1u << i;
+    for (int i = 0; i < 16; ++i) {
+      const int k = (i + tid) & 15;  // the lanes' 16 counts lie 16 banks apart: each starts at another of them
+      if (p + k < P && refs[p + k] <= 0) bits |= 1u << k;
+    }
     int sum;
     int to = found + block_scan(__builtin_popcount(bits), scratch, sum);
     for (; bits; bits &= bits - 1, ++to)
