@@ -286,6 +286,20 @@ def test_tree_without_mask_is_a_piece_of_a_prompt(ops):
     tree_case(ops, 6, [0, 333, 64], [150, 90, 1], 8, 2, 128, 32, mask=False)
 
 
+def test_tree_given_out_and_tokens_outside(ops):
+    """A strided result; q rows in front of the first sequence and behind the last keep what the result held."""
+    g = gen(13)
+    kp, vp, table, ks, vs = paged(g, [70, 33], 32, 2, 64)
+    q = rnd(g, 12, 9, 64)[:, :8]
+    buf = torch.full((12, 9, 64), 5.0, device="cuda")
+    out = ops.attention_tree(q, kp, vp, table, i32([66, 30]), i32([2, 6, 9]), out=buf[:, :8])
+    assert out.data_ptr() == buf.data_ptr()
+    for a, b, n, m in ((2, 0, 4, 70), (6, 1, 3, 33)):
+        want, bound = R.attend(q[a:a + n], ks[b], vs[b], R.causal(n, m))
+        R.check(out[a:a + n], want, bound)
+    assert (buf[:2] == 5.0).all() and (buf[9:] == 5.0).all() and (buf[:, 8] == 5.0).all()
+
+
 def test_tree_empty_rows_give_zeros(ops):
     """No context and no bit: nothing is seen."""
     g = gen(1)

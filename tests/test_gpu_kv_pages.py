@@ -220,6 +220,7 @@ def random_state(rng, B, W, ps, P):
 @pytest.mark.parametrize("B,W,ps,spare,layers,H,D,layout", [
     (1, 1, 16, 4, 1, 1, 64, 0), (8, 6, 16, 5, 2, 2, 64, 0), (40, 9, 32, 30, 1, 1, 96, 1), (33, 20, 16, 200, 3, 1, 64, 2),
     (130, 5, 16, 2, 0, 1, 64, 0),
+    (40, 9, 16, 25000, 1, 1, 64, 0), (1100, 3, 16, 7, 1, 1, 64, 0), (20, 70, 16, 600, 1, 1, 64, 0),
 ])
 def test_assign(ops, seed, B, W, ps, spare, layers, H, D, layout):
     rng = random.Random(seed * 1009 + B)

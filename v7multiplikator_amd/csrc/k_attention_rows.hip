@@ -79,9 +79,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_kernel(A
   const int64_t *words = a.mask + (long long)(s.q0 + tok) * a.mask_words;
   // keys below lim are seen by the row, keys from lim on by the mask's bits or not at all
   const int ctx = min(s.off, s.kv);
-  const int lim = tree ? ctx : clampi(s.off + tok + 1, 0, s.kv);
-  const int lim_min = tree ? ctx : clampi(s.off + row0 / a.group + 1, 0, s.kv);
-  const int lim_max = tree ? s.kv : clampi(s.off + (row0 + n_rows - 1) / a.group + 1, 0, s.kv);
+  const int lim = tree ? ctx : attn_limit(s, tok);
+  const int lim_min = tree ? ctx : attn_limit(s, row0 / a.group);
+  const int lim_max = tree ? s.kv : attn_limit(s, (row0 + n_rows - 1) / a.group);
   const int key_lo = u.piece ? u.piece * u.piece_keys : 0;
   const int key_hi = u.piece + 1 < u.pieces ? min((u.piece + 1) * u.piece_keys, lim_max) : lim_max;
   const int full_hi = min(key_hi, lim_min);  // up to here every row sees every key

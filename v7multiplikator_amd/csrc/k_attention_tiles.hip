@@ -72,9 +72,9 @@ __global__ __launch_bounds__(PAIR ? 512 : 256, D <= 128 ? 2 : 1) void attention_
   const int tok = n_rows ? row / a.group : 0, head = hk * a.group + (n_rows ? row % a.group : 0);
   const bool tree = PAGED && a.mask_words;
   const int64_t *words = a.mask + (long long)(s.q0 + tok) * a.mask_words;
-  auto lim_of = [&](int r) { return clampi(s.off + r / a.group + 1, 0, s.kv); };
+  auto lim_of = [&](int r) { return attn_limit(s, r / a.group); };
   const int ctx = min(s.off, s.kv);
-  const int lim = tree ? ctx : clampi(s.off + tok + 1, 0, s.kv);
+  const int lim = tree ? ctx : attn_limit(s, tok);
   // the wave's rows all see the keys below lim_min, and none from lim_max on
   const int lim_min = tree ? ctx : lim_of(row0);
   const int lim_max = n_rows == 0 ? 0 : (tree ? s.kv : lim_of(row0 + n_rows - 1));

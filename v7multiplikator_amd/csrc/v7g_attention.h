@@ -53,6 +53,12 @@ struct AttnSeq {
 
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
 
+// Keys that token `tok` of a sequence sees under the causal mask.
+__device__ __forceinline__ int attn_limit(const AttnSeq &s, int tok) {
+  const long long n = (long long)s.off + tok + 1;
+  return n < 0 ? 0 : (n > s.kv ? s.kv : (int)n);
+}
+
 template <bool PAGED>
 __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs &a, int b) {
   AttnSeq s;
