@@ -569,7 +569,8 @@ int v7g_kv_pages_compact(const v7g_kv_pages *pages, int32_t *lens_out, const int
  * logprob[t] of token ids[t] (NaN for an id outside the vocabulary), the
  * entropy of the row in nats, and its top_k most likely tokens in order with
  * their log probabilities, [n_tokens, top_k] (0 <= top_k <= 64, top_k <=
- * vocab; equal logits: the lower index first; NaN counts as the largest).
+ * vocab; equal logits, denormals and zeros among them: the lower index
+ * first; NaN counts as the largest).
  * Logits of -inf have probability 0; a row that holds NaN or +inf, or nothing
  * above -inf, has NaN for every probability.  workspace:
  * v7g_token_logprobs_workspace(...) bytes, as for the attention. */

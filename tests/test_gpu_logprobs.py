@@ -106,6 +106,18 @@ def test_ties_fall_to_the_lower_index(ops):
         run(ops, y, torch.tensor([V - 7, 0], dtype=torch.int32, device="cuda"), 30)
 
 
+def test_denormals_count_as_zero(ops):
+    """Denormal logits tie with 0 and -0, whatever their bits: the lower index first."""
+    for V in (500, 9000):
+        x = torch.full((2, V), -1.0, device="cuda")
+        at = [3, 7, 70, 200, 300, V - 1]
+        x[0, at] = torch.tensor([0.0, 1e-40, -1e-41, -0.0, 3e-39, 1e-45], device="cuda")
+        x[1, at] = torch.tensor([-1e-45, 0.0, 1e-38, 2e-39, 0.0, 1.2e-38], device="cuda")
+        ti = ops.token_logprobs(x, some_ids(2, V), 5)[3]
+        assert ti[0].tolist() == at[:5]
+        assert ti[1].tolist() == [V - 1, 3, 7, 70, 200]
+
+
 def test_sorted_rows(ops):
     """Every step of a wave brings better candidates than all before, or none."""
     for V in (3000, 50000):

@@ -5,10 +5,10 @@
 // One pass over the logits, which is what bounds it: each lane keeps its own running maximum and sums (a new maximum
 // scales s and moves w: w' = a (w + s (m - m'))), and each wave the K best of what it has read.  A token is ordered by
 // one 64-bit key, the value's bits made monotonic above the complement of its index, so equal values fall to the
-// lower index, -0 equals 0 and NaN comes first.  A wave reads 1024 logits at a time; those above a bar that K logits are
-// known to reach (first the K-th best of the 64 lanes' best) are collected in LDS, and ranked by counting, which
-// raises the bar, when half as many again have come together and at the end.  A row goes to as many workgroups as fill the chip; a
-// second kernel then joins their results.
+// lower index, -0 and denormals (flushed, as everywhere in this library) equal 0, and NaN comes first.  A wave reads 1024
+// logits at a time; those above a bar that K logits are known to reach (first the K-th best of the 64 lanes' best) are
+// collected in LDS, and ranked by counting, which raises the bar, when half as many again have come together and at the
+// end.  A row goes to as many workgroups as fill the chip; a second kernel then joins their results.
 #include "v7g_device.h"
 #include "v7g_internal.h"
 
@@ -26,7 +26,7 @@ typedef float f4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 // Never 0, which stands for no token.
 __device__ __forceinline__ Key make_key(float x, unsigned index) {
   uint32_t b = __builtin_bit_cast(uint32_t, x);
-  if (b == 0x80000000u) b = 0;
+  if ((b & 0x7f800000u) == 0) b = 0;
   b = (b & 0x7fffffffu) > 0x7f800000u ? 0xffffffffu : ((b & 0x80000000u) ? ~b : b | 0x80000000u);
   return ((Key)b << 32) | (0xffffffffu - index);
 }
@@ -64,7 +64,7 @@ struct Best {
   bool full = false;              // the bar stands
   bool sorted = false;
 
-  // The keys of `hit` lanes join the n that wait.
+  // The keys of the lanes that have one to give join the n that wait.
   __device__ __forceinline__ void push(bool mine, Key k) {
     const unsigned long long hit = __ballot(mine);
     if (!hit) return;
