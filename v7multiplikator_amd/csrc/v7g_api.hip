@@ -962,14 +962,21 @@ AttnPlan attn_plan(int n_seqs, int n_tokens, int group, int n_kv_heads, int head
   p.shift = many ? v7g::kAttnTileShift : v7g::kAttnRowShift;
   const long long tiles = (rows >> p.shift) + n_seqs;
   p.units = tiles;
-  // Units aimed at: four rounds of a workgroup per compute unit (6 trees of up to 60 drafts: 1024 units 116 us, 512
-  // 134, 2048 129; 37 decoded tokens 172, 185, 179), one round of the wide 128-row tiles (4 trees x 256: 256 units
-  // 248 us, 1024 306).  A prompt over its own keys is cut only if its tiles leave half of the chip idle: its longest
-  // tile is twice the mean, and joining costs as much as the tail (2048 tokens, 28/4 heads: whole 93 us, cut 128 to
-  // 180; 512 tokens, 32/8 heads: 29 against 36).
-  const int aim = many && head_dim > 128 ? v7g::kAttnUnits / 4 : v7g::kAttnUnits;
-  if (tiles * n_kv_heads < (self ? v7g::kAttnUnits / 8 : aim) && max_keys > v7g::kAttnMinChunk) {
-    p.target = (aim + n_kv_heads - 1) / n_kv_heads;
+  // Units aimed at: four workgroups for each compute unit (6 trees of up to 60 drafts: 1024 units 100 us, 512 111, 2048
+  // 114; 37 decoded tokens 164, 177, 168), two where a few tiles would be cut in very many pieces, which have to be
+  // joined (2 trees over 16000 keys: 512 units 72 us, 1024 91; one token over 32000: 32 against 34).  Wide heads keep
+  // one workgroup on a compute unit: one round of few rows (4 tokens over 16000 keys, x 256: 256 units 92 us, 512 105,
+  // 1024 112), two of many (4 trees over 8000: 512 units 244 us, 256 379, 1024 298).  Three for each tile at least, so
+  // that long sequences among short ones are cut.
+  const long long whole = tiles * n_kv_heads;
+  long long aim = head_dim > 128 ? (many ? v7g::kAttnUnits / 2 : v7g::kAttnUnits / 4)
+                                 : (whole < 64 ? v7g::kAttnUnits / 2 : v7g::kAttnUnits);
+  if (aim < 3 * whole) aim = 3 * whole < v7g::kAttnUnits ? 3 * whole : v7g::kAttnUnits;
+  // A prompt over its own keys is cut only if its tiles leave half of the chip idle: its longest tile is twice the mean,
+  // and joining costs as much as the tail (2048 tokens, 28/4 heads: whole 93 us, cut 128 to 180; 512 tokens, 32/8 heads:
+  // 29 against 36).
+  if (whole < (self ? v7g::kAttnUnits / 8 : v7g::kAttnUnits) && max_keys > v7g::kAttnMinChunk) {
+    p.target = (int)((aim + n_kv_heads - 1) / n_kv_heads);
     p.units = tiles + p.target;
     p.workspace = ((p.units * n_kv_heads) << p.shift) * (head_dim + 2) * 4;
   }
